@@ -16,7 +16,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libb2attn.so"
 SOURCES = [CSRC / "b2_attn.cu", CSRC / "b2_block.cu", CSRC / "b2_gemm.cu"]
-HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h", CSRC / "b2_internal.h"]
+HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h", CSRC / "b2_internal.h",
+           CSRC / "b2_device.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
