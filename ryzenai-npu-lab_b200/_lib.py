@@ -1,5 +1,4 @@
-"""ctypes binding of libb2attn.so (the C ABI in include/b2_decode_attn.h and
-include/b2_block.h).
+"""ctypes binding of libb2attn.so (the C ABI of the headers in include/).
 
 This module loads the in-tree shared library and nothing else: there is no
 fallback.  If the library is missing or fails to load, every entry point
@@ -178,6 +177,55 @@ SIGNATURES = {
         _p, _i32,            # block_tables, max_blocks_per_seq
         _p, _p, _i32, _i32,  # past_lens, chunk_lens, tokens, batch
         _f32, _p, _p, _p,    # scale, out, dev_err, stream
+    ]),
+    # include/b2_kv8.h
+    "b2_kv8_workspace_bytes": (_i64, []),
+    "b2_kv8_append": (ctypes.c_int, [
+        _p, _i64, _i32,      # qkv, row_stride, rows
+        _p, _p,              # slots, positions
+        _p, _p, _i32,        # past_lens, chunk_lens, tokens
+        _p, _i32,            # block_tables, max_blocks_per_seq
+        _p, _p, _f32,        # gamma_q, gamma_k, eps
+        _p, _p, _i32,        # rope_cos, rope_sin, rope_rows
+        _p, _p, _p, _p, _i32,  # k_pool, v_pool, k_scale, v_scale, num_blocks
+        _p, _i32, _p, _p,    # q_out, mode, dev_err, stream
+    ]),
+    "b2_kv8_decode_step": (ctypes.c_int, [
+        _p, _i64, _i32, _p,  # qkv, row_stride, tokens, chunk_lens
+        _p, _p, _f32,        # gamma_q, gamma_k, eps
+        _p, _p, _i32,        # rope_cos, rope_sin, rope_rows
+        _p, _p, _i32,        # past_lens, block_tables, max_blocks_per_seq
+        _p, _p, _p, _p, _i32,  # k_pool, v_pool, k_scale, v_scale, num_blocks
+        _i32, _f32, _i32, _p,  # batch, scale, mode, out
+        _p, _i64, _p, _p,    # workspace, workspace_bytes, dev_err, stream
+    ]),
+    "b2_kv8_prefill_attn": (ctypes.c_int, [
+        _p, _i64, _i32, _p,  # q, q_stride, rows, row_start
+        _p, _p, _i32,        # past_lens, chunk_lens, tokens
+        _p, _i32,            # block_tables, max_blocks_per_seq
+        _p, _p, _p, _p, _i32,  # k_pool, v_pool, k_scale, v_scale, num_blocks
+        _i32, _f32, _p,      # batch, scale, out
+        _p, _i64, _p, _p,    # workspace, workspace_bytes, dev_err, stream
+    ]),
+    # include/b2_tables.h
+    "b2_tables_extend": (ctypes.c_int, [
+        _p, _i32, _p,        # block_tables, max_blocks_per_seq, held
+        _p, _i32, _p,        # free_list, num_blocks, free_count
+        _p, _p, _i32,        # past_lens, new_lens, batch
+        _p, _p, _p, _p,      # held_out, free_count_out, granted, row_start
+        _p, _p, _i32, _i32,  # slots, positions, rows, tokens_per_seq
+        _p, _p,              # dev_err, stream
+    ]),
+    "b2_slot_map": (ctypes.c_int, [
+        _p, _i32, _i32,      # block_tables, max_blocks_per_seq, num_blocks
+        _p, _p, _p, _i32,    # past_lens, new_lens, row_start, batch
+        _p, _p, _i32, _i32,  # slots, positions, rows, tokens_per_seq
+        _p, _p,              # dev_err, stream
+    ]),
+    "b2_tables_release": (ctypes.c_int, [
+        _p, _i32, _p,        # block_tables, max_blocks_per_seq, held
+        _p, _i32, _p,        # free_list, num_blocks, free_count
+        _p, _i32, _p, _p,    # finished, batch, dev_err, stream
     ]),
     "b2_decode_attn_noalloc": (ctypes.c_int, [
         _p, _p, _p, _i32,    # q, k_pool, v_pool, num_blocks

@@ -1,8 +1,7 @@
 """Build libb2attn.so in-tree with nvcc for sm_100a.
 
 The shared library is the product's compute path: it holds every CUDA kernel
-and the C ABI declared in include/b2_decode_attn.h and include/b2_block.h.  It is built next to this
-file so that it travels with the source tree to the GPU host.
+and the C ABI declared in the headers of include/.  It is built next to this file so that it travels with the source tree to the GPU host.
 """
 from __future__ import annotations
 
@@ -15,8 +14,10 @@ PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libb2attn.so"
-SOURCES = [CSRC / "b2_attn.cu", CSRC / "b2_block.cu", CSRC / "b2_gemm.cu"]
-HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h", CSRC / "b2_internal.h",
+SOURCES = [CSRC / "b2_attn.cu", CSRC / "b2_block.cu", CSRC / "b2_gemm.cu",
+           CSRC / "b2_kv8.cu", CSRC / "b2_tables.cu"]
+HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h",
+           ROOT / "include" / "b2_kv8.h", ROOT / "include" / "b2_tables.h", CSRC / "b2_internal.h",
            CSRC / "b2_device.cuh"]
 
 NVCC_FLAGS = [

@@ -1,0 +1,318 @@
+// Block tables and slot maps built on the GPU (include/b2_tables.h):
+//
+//   extend_kernel   blocks for new tokens off the end of the free list, in
+//                   request order: prefix sums of rows and of needed blocks
+//   slot_kernel     slot and position of every new token's row
+//   release_kernel  blocks of finished requests back to the free list
+//
+// The work is a few bytes per request and eight per row: bound by launch and
+// memory latency, so each call is one or two launches and no thread waits for
+// another CTA.
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+
+#include "b2_decode_attn.h"
+#include "b2_internal.h"
+#include "b2_tables.h"
+
+namespace {
+
+constexpr int kBlock = 64;
+constexpr int kScanThreads = 1024;
+constexpr int kSlotThreads = 256;
+constexpr int32_t kMaxTableWidth = (1 << 25) - 1;  // width x 64 tokens stay an int32
+constexpr int32_t kMaxPoolBlocks = (1 << 22) - 1;
+
+int fail(int code, const char *msg) { return b2_record_error(code, msg); }
+
+// Exclusive prefix sum of `v` over the CTA; `total` gets the CTA's sum.
+__device__ __forceinline__ int64_t scan_exclusive(int64_t v, int64_t *warp_sum, int64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t incl = v;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += u;
+  }
+  __syncthreads();  // warp_sum's last reads are done
+  if (lane == 31) warp_sum[warp] = incl;
+  __syncthreads();
+  int64_t w = lane < kScanThreads / 32 ? warp_sum[lane] : 0;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, w, off);
+    if (lane >= off) w += u;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return incl - v + (warp > 0 ? before : 0);
+}
+
+// Largest i in [0, n) with start[i] <= x, or -1.
+template <class T>
+__device__ __forceinline__ int last_at_or_below(const T *start, int n, T x) {
+  int lo = -1, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+struct ExtendArgs {
+  int32_t *tables;
+  int max_blocks;
+  const int32_t *held, *free_list;
+  int num_blocks;
+  const int32_t *free_count, *past, *fresh;
+  int batch;
+  int32_t *held_out, *count_out, *granted, *row_start;
+  int rows, tokens;
+  int32_t *err;
+};
+
+// One CTA walks the requests, kScanThreads at a time: two prefix sums (rows,
+// needed blocks), then the new table entries of the chunk spread over all
+// threads (an entry finds its request by bisection of the chunk's sums), so
+// one request of many blocks costs no more than many of one.
+__global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a) {
+  __shared__ int64_t warp_sum[kScanThreads / 32];
+  __shared__ int64_t first[kScanThreads];  // exclusive sums of the blocks taken in this chunk
+  __shared__ int32_t from[kScanThreads];   // blocks held before
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int64_t count = a.free_count[0];
+  int flag = 0;
+  if (count < 0 || count > a.num_blocks) {
+    flag = B2_DEV_BAD_LENGTH;
+    count = count < 0 ? 0 : a.num_blocks;
+  }
+  int64_t rows_before = 0, need_before = 0, taken = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kScanThreads) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const bool in = b < a.batch;
+    const int past = in ? a.past[b] : 0, fresh = in ? a.fresh[b] : 0, held = in ? a.held[b] : 0;
+    const int64_t upto = static_cast<int64_t>(past) + fresh;
+    bool bad = past < 0 || fresh < 0 || held < 0 || held > a.max_blocks ||
+               upto > static_cast<int64_t>(a.max_blocks) * kBlock || (a.tokens > 0 && fresh > a.tokens);
+    int64_t total = 0;
+    int64_t start = static_cast<int64_t>(b) * a.tokens;
+    if (a.tokens == 0) {
+      const int64_t n = fresh > 0 ? fresh : 0;
+      start = rows_before + scan_exclusive(n, warp_sum, total);
+      rows_before += total;
+      if (n > 0 && start + n > a.rows) bad = true;
+    }
+    if (bad) flag = B2_DEV_BAD_LENGTH;
+    const int64_t blocks = (upto + kBlock - 1) / kBlock;
+    const int64_t need = in && !bad && blocks > held ? blocks - held : 0;
+    const int64_t pre = need_before + scan_exclusive(need, warp_sum, total);
+    need_before += total;
+    const bool ok = !bad && (need == 0 || pre + need <= count);
+    const int64_t take = ok ? need : 0;
+    int64_t chunk = 0;
+    const int64_t pos = scan_exclusive(take, warp_sum, chunk);
+    first[threadIdx.x] = pos;
+    from[threadIdx.x] = held;
+    __syncthreads();
+    for (int64_t e = threadIdx.x; e < chunk; e += kScanThreads) {
+      const int i = last_at_or_below<int64_t>(first, kScanThreads, e);
+      int id = a.free_list[count - 1 - (taken + e)];
+      if (id < 0 || id >= a.num_blocks) {
+        flag |= B2_DEV_BAD_BLOCK;
+        id = -1;
+      }
+      a.tables[static_cast<int64_t>(b0 + i) * a.max_blocks + from[i] + (e - first[i])] = id;
+    }
+    taken += chunk;
+    if (in) {
+      a.held_out[b] = held + static_cast<int32_t>(take);
+      a.granted[b] = ok ? fresh : 0;
+      a.row_start[b] = static_cast<int32_t>(start < a.rows ? start : a.rows);
+    }
+    __syncthreads();
+  }
+  if (flag) atomicOr(a.err, flag);
+  if (threadIdx.x == 0) a.count_out[0] = static_cast<int32_t>(count - taken);
+}
+
+struct SlotArgs {
+  const int32_t *tables;
+  int max_blocks, num_blocks;
+  const int32_t *past, *fresh, *granted, *row_start;
+  int batch;
+  int32_t *slots, *positions;
+  int rows, tokens;
+  int32_t *err;  // NULL: faults were reported before
+};
+
+// One thread per row; packed rows find their request by bisection.
+__global__ void __launch_bounds__(kSlotThreads) slot_kernel(const SlotArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x;
+  if (r >= a.rows) return;
+  int b;
+  if (a.tokens > 0 && !a.row_start) b = static_cast<int>(r / a.tokens);
+  else b = last_at_or_below<int32_t>(a.row_start, a.batch, static_cast<int32_t>(r));
+  int slot = -1, position = 0;
+  if (b >= 0 && b < a.batch) {
+    const int64_t start = a.row_start ? a.row_start[b] : static_cast<int64_t>(b) * a.tokens;
+    const int64_t t = r - start;
+    if (t < a.fresh[b]) {
+      const int64_t pos = a.past[b] + t;
+      position = static_cast<int>(pos);
+      int flag = 0;
+      if (!a.granted || a.granted[b] > 0) {
+        if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) {
+          flag = B2_DEV_BAD_LENGTH;
+        } else {
+          const int blk = a.tables[static_cast<int64_t>(b) * a.max_blocks + pos / kBlock];
+          if (blk < 0 || blk >= a.num_blocks) flag = B2_DEV_BAD_BLOCK;
+          else slot = blk * kBlock + static_cast<int>(pos % kBlock);
+        }
+      }
+      if (flag && a.err) atomicOr(a.err, flag);
+    }
+  }
+  a.slots[r] = slot;
+  a.positions[r] = position;
+}
+
+struct ReleaseArgs {
+  int32_t *tables;
+  int max_blocks;
+  int32_t *held, *free_list;
+  int num_blocks;
+  int32_t *free_count;
+  const uint8_t *finished;
+  int batch;
+  int32_t *err;
+};
+
+__global__ void __launch_bounds__(kScanThreads) release_kernel(const ReleaseArgs a) {
+  __shared__ int64_t warp_sum[kScanThreads / 32];
+  __shared__ int64_t first[kScanThreads];
+  const int64_t count = a.free_count[0];
+  // first the sum over all requests: nothing is released that does not fit
+  int64_t mine = 0, sum = 0;
+  bool bad = count < 0;
+  for (int b = threadIdx.x; b < a.batch; b += kScanThreads)
+    if (a.finished[b]) {
+      const int h = a.held[b];
+      if (h < 0 || h > a.max_blocks) bad = true;
+      else mine += h;
+    }
+  scan_exclusive(mine, warp_sum, sum);
+  bad = __syncthreads_or(bad) || count + sum > a.num_blocks;
+  if (bad) {
+    if (threadIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+    return;
+  }
+  int64_t at = count;
+  for (int b0 = 0; b0 < a.batch; b0 += kScanThreads) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const int64_t n = b < a.batch && a.finished[b] ? a.held[b] : 0;
+    int64_t chunk = 0;
+    first[threadIdx.x] = scan_exclusive(n, warp_sum, chunk);
+    __syncthreads();
+    for (int64_t e = threadIdx.x; e < chunk; e += kScanThreads) {
+      const int i = last_at_or_below<int64_t>(first, kScanThreads, e);
+      int32_t *entry = a.tables + static_cast<int64_t>(b0 + i) * a.max_blocks + (e - first[i]);
+      a.free_list[at + e] = *entry;
+      *entry = -1;
+    }
+    if (n > 0) a.held[b] = 0;
+    at += chunk;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) a.free_count[0] = static_cast<int32_t>(at);
+}
+
+int launched(cudaError_t e, const char *what) {
+  const cudaError_t sticky = cudaGetLastError();
+  if (e == cudaSuccess) e = sticky;
+  if (e == cudaSuccess) return b2_clear_error();
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s launch failed: %s", what, cudaGetErrorString(e));
+  return fail(B2_ERR_CUDA, msg);
+}
+
+// `dependent`: after extend_kernel, whose launch it overlaps.
+int launch_slots(const SlotArgs &a, bool dependent, cudaStream_t st) {
+  if (a.rows == 0) return b2_clear_error();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(a.rows) + kSlotThreads - 1) / kSlotThreads));
+  cfg.blockDim = dim3(kSlotThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return launched(cudaLaunchKernelEx(&cfg, slot_kernel, a), "slot_kernel");
+}
+
+int check_sizes(int32_t max_blocks, int32_t num_blocks, int32_t batch, int32_t rows, int32_t tokens) {
+  if (batch < 0 || rows < 0 || tokens < 0) return fail(B2_ERR_ARG, "batch, rows and tokens_per_seq must be >= 0");
+  if (max_blocks <= 0 || max_blocks > kMaxTableWidth)
+    return fail(B2_ERR_ARG, "max_blocks_per_seq must be in [1, 2^25)");
+  if (num_blocks <= 0 || num_blocks > kMaxPoolBlocks) return fail(B2_ERR_ARG, "num_blocks must be in [1, 2^22)");
+  if (tokens > 0 && static_cast<int64_t>(batch) * tokens != rows)
+    return fail(B2_ERR_ARG, "rows must be batch * tokens_per_seq");
+  return B2_OK;
+}
+
+}  // namespace
+
+extern "C" int b2_tables_extend(int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *held,
+                                const int32_t *free_list, int32_t num_blocks, const int32_t *free_count,
+                                const int32_t *past_lens, const int32_t *new_lens, int32_t batch, int32_t *held_out,
+                                int32_t *free_count_out, int32_t *granted, int32_t *row_start, int32_t *slots,
+                                int32_t *positions, int32_t rows, int32_t tokens_per_seq, int32_t *dev_err,
+                                void *stream) {
+  const int rc = check_sizes(max_blocks_per_seq, num_blocks, batch, rows, tokens_per_seq);
+  if (rc) return rc;
+  if (!free_list || !free_count || !free_count_out || !dev_err ||
+      (batch > 0 && (!block_tables || !held || !past_lens || !new_lens || !held_out || !granted || !row_start)) ||
+      (rows > 0 && (!slots || !positions)))
+    return fail(B2_ERR_ARG, "b2_tables_extend: null pointer argument");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  ExtendArgs a{block_tables, max_blocks_per_seq, held, free_list, num_blocks, free_count, past_lens, new_lens, batch,
+               held_out, free_count_out, granted, row_start, rows, tokens_per_seq, dev_err};
+  extend_kernel<<<1, kScanThreads, 0, st>>>(a);
+  const int lrc = launched(cudaSuccess, "extend_kernel");
+  if (lrc) return lrc;
+  SlotArgs s{block_tables, max_blocks_per_seq, num_blocks, past_lens, new_lens, granted,
+             tokens_per_seq > 0 ? nullptr : row_start, batch, slots, positions, rows, tokens_per_seq, nullptr};
+  return launch_slots(s, true, st);
+}
+
+extern "C" int b2_slot_map(const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t num_blocks,
+                           const int32_t *past_lens, const int32_t *new_lens, const int32_t *row_start, int32_t batch,
+                           int32_t *slots, int32_t *positions, int32_t rows, int32_t tokens_per_seq, int32_t *dev_err,
+                           void *stream) {
+  const int rc = check_sizes(max_blocks_per_seq, num_blocks, batch, rows, row_start ? 0 : tokens_per_seq);
+  if (rc) return rc;
+  if (!row_start && tokens_per_seq <= 0 && rows > 0)
+    return fail(B2_ERR_ARG, "b2_slot_map: row_start or tokens_per_seq > 0 is required");
+  if (rows == 0) return b2_clear_error();
+  if (!slots || !positions || !dev_err || (batch > 0 && (!block_tables || !past_lens || !new_lens)))
+    return fail(B2_ERR_ARG, "b2_slot_map: null pointer argument");
+  SlotArgs s{block_tables, max_blocks_per_seq, num_blocks, past_lens, new_lens, nullptr, row_start, batch,
+             slots, positions, rows, row_start ? 0 : tokens_per_seq, dev_err};
+  return launch_slots(s, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b2_tables_release(int32_t *block_tables, int32_t max_blocks_per_seq, int32_t *held, int32_t *free_list,
+                                 int32_t num_blocks, int32_t *free_count, const uint8_t *finished, int32_t batch,
+                                 int32_t *dev_err, void *stream) {
+  const int rc = check_sizes(max_blocks_per_seq, num_blocks, batch, 0, 0);
+  if (rc) return rc;
+  if (batch == 0) return b2_clear_error();
+  if (!block_tables || !held || !free_list || !free_count || !finished || !dev_err)
+    return fail(B2_ERR_ARG, "b2_tables_release: null pointer argument");
+  ReleaseArgs a{block_tables, max_blocks_per_seq, held, free_list, num_blocks, free_count, finished, batch, dev_err};
+  release_kernel<<<1, kScanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launched(cudaSuccess, "release_kernel");
+}

@@ -88,16 +88,18 @@ class PagedKVCache:
         self.num_layers = num_layers
         self.device = torch.device(device)
         self.max_blocks = blocks_for(capacity_tokens)
-        shape = (num_layers, num_blocks, HKV, BLOCK, D)
+        self._allocate((num_layers, num_blocks, HKV, BLOCK, D), fill)
+        self.allocator = BlockAllocator(num_blocks, shuffle_seed)
+        self._tables: list[list[int]] = []
+        self.lengths: list[int] = []
+
+    def _allocate(self, shape, fill: float | None) -> None:
         if fill is None:
             self.k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
             self.v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         else:
             self.k = torch.full(shape, fill, dtype=torch.bfloat16, device=self.device)
             self.v = torch.full(shape, fill, dtype=torch.bfloat16, device=self.device)
-        self.allocator = BlockAllocator(num_blocks, shuffle_seed)
-        self._tables: list[list[int]] = []
-        self.lengths: list[int] = []
 
     @property
     def batch(self) -> int:
@@ -158,3 +160,81 @@ class PagedKVCache:
         k = kp[ids].transpose(0, 1).reshape(HKV, nb * BLOCK, D)[:, :length]
         v = vp[ids].transpose(0, 1).reshape(HKV, nb * BLOCK, D)[:, :length]
         return k, v
+
+
+KV8_MAX = 448.0              # the largest e4m3 code
+KV8_MIN_SCALE = 2.0 ** -100
+
+
+def kv8_scale(amax: torch.Tensor) -> torch.Tensor:
+    """The scale of a (block, head) whose largest magnitude is `amax` (finite,
+    >= 0): the smallest power of two s >= 2^-100 with amax <= 448 * s."""
+    m, e = torch.frexp(amax.float() / KV8_MAX)
+    s = torch.ldexp(torch.ones_like(m), torch.where(m == 0.5, e - 1, e))
+    return torch.where(amax > 0, s, torch.zeros_like(s)).clamp(min=KV8_MIN_SCALE)
+
+
+class PagedKVCache8(PagedKVCache):
+    """PagedKVCache in 8 bits: e4m3 codes with a power-of-two fp32 scale for
+    each block and KV head, half the bytes of the bf16 cache.
+
+        k        float8_e4m3fn [layers, num_blocks, 8, 64 tokens, 64 dims]
+        v        float8_e4m3fn [layers, num_blocks, 8, 64 dims, 64 tokens]
+        k_scale, v_scale       float32 [layers, num_blocks, 8]
+
+    attention_kv8 appends to it and attends over it; the bf16 kernels refuse
+    it.  Block allocation and tables are PagedKVCache's."""
+
+    def _allocate(self, shape, fill: float | None) -> None:
+        layers, blocks = shape[:2]
+        tiles = (layers, blocks, HKV, BLOCK * D)
+
+        def codes():
+            if fill is None:
+                return torch.empty(tiles, dtype=torch.float8_e4m3fn, device=self.device)
+            return torch.full(tiles, fill, dtype=torch.float32).to(torch.float8_e4m3fn).to(self.device)
+        self.k = codes().view(layers, blocks, HKV, BLOCK, D)
+        self.v = codes().view(layers, blocks, HKV, D, BLOCK)
+        value = 1.0 if fill is None else fill
+        self.k_scale = torch.full((layers, blocks, HKV), value, dtype=torch.float32, device=self.device)
+        self.v_scale = torch.full((layers, blocks, HKV), value, dtype=torch.float32, device=self.device)
+
+    def kv8(self, layer: int = 0) -> dict[str, torch.Tensor]:
+        """The layer's pools and scales under the names attention_kv8 takes."""
+        return {"k_pool": self.k[layer], "v_pool": self.v[layer], "k_scale": self.k_scale[layer],
+                "v_scale": self.v_scale[layer]}
+
+    def write_dense(self, layer: int, seq: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Quantise a dense [8, T, 64] history into the sequence's blocks (set-up,
+        not the decode path): what one append of the T tokens to the empty
+        sequence stores."""
+        t = k.shape[1]
+        nb = blocks_for(t)
+        if nb > len(self._tables[seq]):
+            raise ValueError("history longer than the sequence's capacity")
+        if nb == 0:
+            return
+        ids = torch.tensor(self._tables[seq][:nb], device=self.device)
+        pad = nb * BLOCK - t
+        for x, pool, scale, dim_major in ((k, self.k, self.k_scale, False), (v, self.v, self.v_scale, True)):
+            x = torch.nn.functional.pad(x.to(self.device, torch.bfloat16).float(), (0, 0, 0, pad))
+            x = x.reshape(HKV, nb, BLOCK, D).transpose(0, 1)
+            big = torch.finfo(torch.bfloat16).max
+            x = x.clamp(-big, big)
+            s = kv8_scale(x.abs().nan_to_num(0.0).amax((2, 3)))
+            c = (x / s[..., None, None]).to(torch.float8_e4m3fn)
+            c = c.transpose(2, 3) if dim_major else c
+            pool[layer].view(torch.uint8)[ids] = c.contiguous().view(torch.uint8)
+            scale[layer][ids] = s
+
+    def read_dense(self, layer: int, seq: int, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """[8, length, 64] bf16 K and V of one sequence, the values its codes
+        stand for (bf16 holds a code times its scale exactly)."""
+        nb = blocks_for(length)
+        ids = torch.tensor(self._tables[seq][:nb], device=self.device, dtype=torch.long)
+        out = []
+        for pool, scale, dim_major in ((self.k, self.k_scale, False), (self.v, self.v_scale, True)):
+            x = pool[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float() * scale[layer][ids][..., None, None]
+            x = x.transpose(2, 3) if dim_major else x
+            out.append(x.transpose(0, 1).reshape(HKV, nb * BLOCK, D)[:, :length].to(torch.bfloat16))
+        return out[0], out[1]
