@@ -400,24 +400,33 @@ __global__ void __launch_bounds__(128) kv8_attn_kernel(const AttnArgs a) {
 // so every warp streams the same number of tiles whatever the lengths are.  A
 // warp is its own pipeline: lane 0 copies the tiles of the warp's range
 // (cp.async.bulk on an mbarrier per stage) kStages ahead, the warp multiplies
-// them with mma.sync m16n8k16 in f16 (e4m3 codes are exact in f16) and hands
-// the stage back to itself, with no barrier between warps until the end.
+// them on the tensor cores and hands the stage back to itself, with no barrier
+// between warps until the end.
 //
-//   S[64 x 8]   = K[64 x 64] . Q^T       columns: new token x head of the pair
-//   O^T[64 x 8] += V^T[64 x 64] . P^T    V is stored dim-major, so both A
-//                                        operands are rows of 16-byte pieces
+//   S[64 x 8]   = K[64 x 64] . Q^T       columns: (new token, head of the pair)
+//   O^T[64 x 8] += V^T[64 x 64] . P^T    V is stored dim-major, so both A operands
+//                                        are rows of 16-byte pieces
+// The products are mma.sync m16n8k16 in f16, which holds every e4m3 code
+// exactly.  (mma.sync m16n8k32 on the codes themselves runs at 0.4 of that rate
+// per element here and needs Q and P in two parts: 60.5 us against 57.4 us for
+// 64 sequences of 128-8192 tokens.)  Vector v (2 * new token + head) is column
+// 2 v, or 2 (v - 4) + 1: a lane then holds the scores of one vector, of two only
+// with 3 or 4 new tokens.
+//
 // Which tokens and dims the rows and k slots of a fragment stand for is free as
-// long as both operands agree: a lane's 16 k slots of four mma steps are 16
+// long as both operands agree: a lane's 16 k slots of two mma steps are 16
 // adjacent bytes of a row, so an operand of 16 rows is two 16-byte loads per
 // lane, free of bank conflicts without a swizzle.
 //
-// Scales: a column's scores are c * (q factor * k scale).  The sum of p runs
-// against the reference m (log2 units), moved only when a score exceeds m + 8
-// (a vote, no shuffles, in all other tiles).  The products p * v scale are
-// rounded to f16 against a reference of their own, mo: g = v scale * 2^(m -
-// mo) <= 2^7 keeps p * g below 2^15; above that the tile's true maximum
-// decides whether mo moves.  f16 holds 11 bits of p (bf16 would hold 8) down to
-// 2^-14 of the reference.
+// Scales: a vector's scores are c * (q factor * k scale), the query scaled to
+// 2^8 so that f16 keeps all bf16 bits of values down to 2^-22 of its largest.
+// The sum of p runs against the reference m (log2 units), moved only when a
+// score exceeds m + kSlack (a vote, no shuffles, in all other tiles).  The
+// products p * v scale are rounded to f16 against a reference of their own, mo:
+// g = v scale * 2^(m - mo) is 1 where the largest product so far is 1, and up to
+// kMaxGain needs no look at the tile (p * g <= 2^15); above, the tile's true
+// maximum decides whether mo moves.  f16 gives p 11 bits (bf16 would give 8)
+// down to 2^-14 of the largest product; what is below 2^-25 of it is lost.
 //
 // Ends: a segment (sequence, head) inside one warp's range is written by that
 // warp.  Others leave partial states in shared memory, merged by the CTA after
@@ -425,37 +434,46 @@ __global__ void __launch_bounds__(128) kv8_attn_kernel(const AttnArgs a) {
 // CTA to arrive merges it in CTA order (the result does not depend on who is
 // last).  At most two segments of a CTA are open, so the workspace has two
 // slots and one counter per CTA whatever the batch.
-constexpr int kStages = 3;
-constexpr int kWarps = 8;
-constexpr int kStepThreads = kWarps * 32;
-constexpr int kMaxSeqs = 2048;   // sequences per launch (prefix sums in shared memory)
+template <int kT>
+constexpr int step_warps() { return kT <= 2 ? 12 : 10; }
+template <int kT>
+constexpr int step_stages() { return 2; }
+constexpr int kMaxSeqs = 1024;   // sequences per launch (lengths and sums in shared memory)
+constexpr int kSegmentCost = 2;  // tiles that the start and end of a segment weigh as
 constexpr int kMaxCtas = 256;
 constexpr uint64_t kDrainNs = 2000000000ull;
-constexpr float kSlack = 8.0f;          // log2 units that p may exceed 1 by
+constexpr float kSlack = 8.0f;          // log2 units that a score may exceed m by
 constexpr float kMaxGain = 128.0f;      // g without a look at the tile's maximum
 constexpr float kUnset = -1.0e30f;
 
 template <int kT>
 struct __align__(128) StepShared {
-  static constexpr int kCols = 2 * kT;
-  struct State {  // unnormalised output, then (m, l), of every column
-    float o[kCols][kDim];
-    float ml[kCols][2];
+  static constexpr int kWarps = step_warps<kT>(), kStages = step_stages<kT>();
+  static constexpr int kSets = (kT + 1) / 2;  // vectors of a lane
+  static constexpr int kVecs = 4 * kSets;     // vectors: 2 * new token + head of the pair
+  struct State {  // unnormalised output, then (m, l), of every vector
+    float o[kVecs][kDim];
+    float ml[kVecs][2];
   };
   uint8_t codes[kWarps][kStages][2 * kTile];
-  float scales[kWarps][kStages][8];  // k scales of 4 adjacent heads, v scales
   union {
-    uint16_t q[8][kDim];             // f16, scaled per column
-    uint16_t out[8][kDim];           // bf16, on the way to memory
+    uint16_t q[kVecs][kDim];         // f16, scaled
+    uint16_t out[kVecs][kDim];       // bf16, on the way to memory
   } row[kWarps];
   State head[kWarps];                // a segment that began before the warp's range
-  float factor[kWarps][8];
+  float factor[kWarps][kVecs];
   uint64_t full[kWarps][kStages];
   int tile[kWarps][kStages];         // block * 8 + head, -1: no such block
   int open[kWarps][2];               // segments of the warp's partial states (head[], codes[][0]), -1: none
   int warp_sum[kWarps];
-  int prefix[kMaxSeqs + 1];          // blocks of sequences 0 .. b-1
+  int pos[kMaxSeqs + 1];             // where a sequence's work starts
+  int past[kMaxSeqs];
+  uint8_t fresh[kMaxSeqs];           // new tokens
 };
+
+static_assert(sizeof(StepShared<2>) + 128 <= 232448 && sizeof(StepShared<kMaxStepTokens>) + 128 <= 232448,
+              "shared memory of a CTA");
+static_assert(2 * step_warps<2>() <= 32 && 2 * step_warps<kMaxStepTokens>() <= 32, "open states fit a bit mask");
 
 struct StepArgs {
   const uint16_t *qkv;
@@ -474,7 +492,7 @@ struct StepArgs {
   float scale_log2;
   int mode;
   uint16_t *out;
-  int32_t *counters;  // [kMaxCtas], zero between calls
+  int32_t *counters;  // [kMaxCtas][kMaxStepTokens], zero between calls
   float *slots;       // [kMaxCtas][2] states
   int32_t *err;
   uint64_t wait_ns;
@@ -515,76 +533,72 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// A 16 x 64 operand of codes: this lane's 16 bytes of rows g and g + 8.
-__device__ __forceinline__ void mma_codes(float c[4], const uint4 &r0, const uint4 &r1, const uint32_t b[4][2]) {
-  const uint32_t u[4] = {r0.x, r0.y, r0.z, r0.w}, w[4] = {r1.x, r1.y, r1.z, r1.w};
+// The product of a 64 x 64 operand of codes with 64 x 8 columns: r[i] are this
+// lane's 16 bytes of rows g and g + 8 of m-tile i.  The four m-tiles take turns,
+// so four independent products are in flight.
+__device__ __forceinline__ void mma_codes(float c[4][4], const uint4 r[4][2], const uint32_t b[4][2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t a0, a1, a2, a3;
-    codes_f16(u[i], a0, a2);
-    codes_f16(w[i], a1, a3);
-    mma_f16(c, a0, a1, a2, a3, b[i][0], b[i][1]);
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = k == 0 ? r[i][0].x : k == 1 ? r[i][0].y : k == 2 ? r[i][0].z : r[i][0].w;
+      const uint32_t w = k == 0 ? r[i][1].x : k == 1 ? r[i][1].y : k == 2 ? r[i][1].z : r[i][1].w;
+      uint32_t a0, a1, a2, a3;
+      codes_f16(u, a0, a2);
+      codes_f16(w, a1, a3);
+      mma_f16(c[i], a0, a1, a2, a3, b[k][0], b[k][1]);
+    }
   }
 }
 
-// First tile of unit u of `units` over `total` tiles.
-__device__ __forceinline__ int unit_start(int u, int total, int units) {
-  return static_cast<int>(static_cast<int64_t>(u) * total / units);
-}
-
-// Running sum of partial states: lane (16 lanes per column) owns columns 2 v +
-// lane / 16 and 4 dims of each.
-template <int kT>
+// Sum of partial states of one new token: 16 lanes per head of the pair, 4 dims
+// each.  States come in groups of 16, lane i of the 16 holding state i's (m, l).
 struct StateSum {
-  float m[kT], l[kT];
-  float4 o[kT];
-  __device__ __forceinline__ void clear() {
+  float m = kUnset, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float c = 0.f;  // factor of this lane's state of the group
+  __device__ __forceinline__ void group(float2 ml) {
+    float top = ml.x;
 #pragma unroll
-    for (int v = 0; v < kT; ++v) {
-      m[v] = kUnset;
-      l[v] = 0.f;
-      o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
-  __device__ __forceinline__ void add(int v, float2 ml, float4 x) {
-    const float n = fmaxf(m[v], ml.x);
-    const float c0 = ex2(m[v] - n), c1 = ex2(ml.x - n);
-    m[v] = n;
-    l[v] = l[v] * c0 + ml.y * c1;
-    o[v].x = o[v].x * c0 + x.x * c1;
-    o[v].y = o[v].y * c0 + x.y * c1;
-    o[v].z = o[v].z * c0 + x.z * c1;
-    o[v].w = o[v].w * c0 + x.w * c1;
-  }
-  __device__ __forceinline__ void store(typename StepShared<kT>::State *to, int lane) const {
-    const int d = 4 * (lane & 15);
+    for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    const float n = fmaxf(m, top), again = ex2(m - n);
+    m = n;
+    c = ex2(ml.x - n);
+    float s = ml.y * c;
 #pragma unroll
-    for (int v = 0; v < kT; ++v) {
-      const int col = 2 * v + (lane >> 4);
-      *reinterpret_cast<float4 *>(&to->o[col][d]) = o[v];
-      if (d == 0) *reinterpret_cast<float2 *>(to->ml[col]) = make_float2(m[v], l[v]);
-    }
+    for (int off = 1; off < 16; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    l = fmaf(l, again, s);
+    o.x *= again;
+    o.y *= again;
+    o.z *= again;
+    o.w *= again;
   }
-  // the context rows of `ntok` tokens, kHq * kDim apart
-  __device__ __forceinline__ void write(uint16_t *out, int ntok, int lane) const {
-#pragma unroll
-    for (int v = 0; v < kT; ++v) {
-      if (v >= ntok) break;
-      const float inv = 1.0f / l[v];
-      *reinterpret_cast<uint2 *>(out + (v * kHq + (lane >> 4)) * kDim + 4 * (lane & 15)) =
-          make_uint2(pack_bf16x2_rn(o[v].x * inv, o[v].y * inv), pack_bf16x2_rn(o[v].z * inv, o[v].w * inv));
-    }
+  __device__ __forceinline__ void add(int i, float4 x, int lane) {
+    const float f = __shfl_sync(0xffffffffu, c, (lane & 16) + i);
+    o.x = fmaf(x.x, f, o.x);
+    o.y = fmaf(x.y, f, o.y);
+    o.z = fmaf(x.z, f, o.z);
+    o.w = fmaf(x.w, f, o.w);
+  }
+  // the two context rows
+  __device__ __forceinline__ void write(uint16_t *out, int lane) const {
+    const float inv = 1.0f / l;
+    *reinterpret_cast<uint2 *>(out + (lane >> 4) * kDim + 4 * (lane & 15)) =
+        make_uint2(pack_bf16x2_rn(o.x * inv, o.y * inv), pack_bf16x2_rn(o.z * inv, o.w * inv));
   }
 };
 
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+
 template <int kT>
-__global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(const StepArgs a) {
   using Shared = StepShared<kT>;
   using State = typename Shared::State;
+  constexpr int kWarps = Shared::kWarps, kStages = Shared::kStages, kStepThreads = kWarps * 32;
   extern __shared__ uint8_t smem_raw[];
   Shared &sh = *reinterpret_cast<Shared *>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;   // mma: row (column) group, thread in group
+  const int g = lane >> 2, t = lane & 3;    // mma: row (column) group, thread in group
   const int j = lane & 7, grp = lane >> 3;  // head vectors: 8 values, vector of four
   if (lane == 0) {
 #pragma unroll
@@ -595,21 +609,21 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // blocks of every sequence, and their prefix sums
-  auto lengths = [&](int b, int &past, int &ntok) -> bool {
-    past = __ldg(a.past_lens + b);
-    ntok = a.chunk_lens ? __ldg(a.chunk_lens + b) : a.tokens;
-    return past >= 0 && ntok >= 0 && ntok <= a.tokens &&
-           static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock;
-  };
+  // The batch's work as a line: sequence b has the positions [pos[b], pos[b + 1]),
+  // its 8 heads' segments in turn, a segment its tiles and kSegmentCost more
+  // positions that stand for the cost of its start and end.
   int running = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kStepThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
     int n = 0;
     if (b < a.batch) {
-      int past, ntok;
-      if (lengths(b, past, ntok)) n = ntok > 0 ? (past + ntok + kBlock - 1) / kBlock : 0;
-      else if (blockIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+      const int past = __ldg(a.past_lens + b), ntok = a.chunk_lens ? __ldg(a.chunk_lens + b) : a.tokens;
+      const bool fits = past >= 0 && ntok >= 0 && ntok <= a.tokens &&
+                        static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock;
+      if (!fits && blockIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+      if (fits && ntok > 0) n = ((past + ntok + kBlock - 1) / kBlock + kSegmentCost) * kHkv;
+      sh.past[b] = past;
+      sh.fresh[b] = static_cast<uint8_t>(n > 0 ? ntok : 0);
     }
     int incl = n;
 #pragma unroll
@@ -619,99 +633,140 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
     }
     if (lane == 31) sh.warp_sum[warp] = incl;
     __syncthreads();
-    int before = running, all = 0;
+    int before = running;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const int v = sh.warp_sum[w];
-      before += w < warp ? v : 0;
-      all += v;
+      if (w < warp) before += v;
+      running += v;
     }
-    if (b < a.batch) sh.prefix[b + 1] = before + incl;
-    running += all;
+    if (b < a.batch) sh.pos[b + 1] = before + incl;
+    if (threadIdx.x == 0 && b0 == 0) sh.pos[0] = 0;
     __syncthreads();
   }
-  if (threadIdx.x == 0) sh.prefix[0] = 0;
-  __syncthreads();
-  const int total = running * kHkv;
-  // as many CTAs as there are warps' tiles to hand out
-  const int ctas = min(static_cast<int>(gridDim.x), (total + kWarps - 1) / kWarps);
+  const int weight = running;
+  // as many CTAs as there are positions for their warps
+  const int ctas = min(static_cast<int>(gridDim.x), (weight + kWarps - 1) / kWarps);
   if (static_cast<int>(blockIdx.x) >= ctas) return;
-  const int units = ctas * kWarps, unit = static_cast<int>(blockIdx.x) * kWarps + warp;
-  const int x0 = unit_start(unit, total, units), x1 = unit_start(unit + 1, total, units);
+  // this warp's positions [w0, w1): lane 0 and 1 divide
+  const int unit = static_cast<int>(blockIdx.x) * kWarps + warp;
+  const int edge = static_cast<int>(static_cast<uint64_t>(unit + (lane & 1)) * static_cast<uint32_t>(weight) /
+                                    static_cast<uint32_t>(ctas * kWarps));
+  const int w0 = __shfl_sync(0xffffffffu, edge, 0), w1 = __shfl_sync(0xffffffffu, edge, 1);
 
-  // the sequence that block number p of the batch belongs to
-  auto sequence_of = [&](int p) {
+  // sequence, head, block of position w; a block past the segment's last stands for its cost
+  auto place = [&](int w, int &sb, int &head, int &block, int &blocks) {
     int lo = 0, hi = a.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (sh.prefix[mid] <= p) lo = mid; else hi = mid;
+      if (sh.pos[mid] <= w) lo = mid; else hi = mid;
     }
-    return lo;
+    const int start = sh.pos[lo], per = (sh.pos[lo + 1] - start) / kHkv;
+    sb = lo;
+    head = (w - start) / per;
+    block = w - start - head * per;
+    blocks = per - kSegmentCost;
   };
-  // pool tile of tile number x (table entry read by this lane), -1: no such block
-  auto pool_tile = [&](int x) {
-    if (x >= x1) return -1;
-    const int b = sequence_of(x / kHkv);
-    const int n = sh.prefix[b + 1] - sh.prefix[b], r = x - sh.prefix[b] * kHkv;
-    const int h = r / n;
-    const int blk = __ldg(a.block_tables + static_cast<int64_t>(b) * a.max_blocks + (r - h * n));
-    return blk < 0 || blk >= a.num_blocks ? -1 : blk * kHkv + h;
+  constexpr int kNoTile = -2;  // a position without a tile; -1: a tile without a valid block
+  int b = 0, h = 0, blk = 0, nblk = 0;
+  auto look = [&](int w, bool keep) {
+    int sb = 0, head = 0, block = 0, blocks = 0, id = kNoTile;
+    if (w < w1) {
+      place(w, sb, head, block, blocks);
+      if (block < blocks) {
+        const int e = __ldg(a.block_tables + static_cast<int64_t>(sb) * a.max_blocks + block);
+        id = e < 0 || e >= a.num_blocks ? -1 : e * kHkv + head;
+      }
+    }
+    if (keep) {  // the warp starts at lane 0's position
+      b = __shfl_sync(0xffffffffu, sb, 0);
+      h = __shfl_sync(0xffffffffu, head, 0);
+      blk = __shfl_sync(0xffffffffu, block, 0);
+      nblk = __shfl_sync(0xffffffffu, blocks, 0);
+    }
+    return id;
   };
 
   const uint64_t policy = evict_first_policy();
-  int entry = pool_tile(x0 + lane), entry_next = pool_tile(x0 + 32 + lane);  // of 32 tiles of the range each
-  int issued = 0;
+  // tiles of 32 positions: one per lane, those not issued yet in `left`
+  int base = w0, entry = look(w0 + lane, true), entry_next = kNoTile, issued = 0;
+  uint32_t left = __ballot_sync(0xffffffffu, entry != kNoTile);
+  bool looked = false;  // entry_next is the next 32 positions
+  float2 scales[kStages];  // k and v scale of the tiles in flight, the next one's first
   auto issue = [&]() {
-    if (x0 + issued >= x1) return;
-    if (issued > 0 && (issued & 31) == 0) {
-      entry = entry_next;
-      entry_next = pool_tile(x0 + issued + 32 + lane);
+    while (left == 0) {
+      if (base + 32 >= w1) return;
+      base += 32;
+      entry = looked ? entry_next : look(base + lane, false);
+      looked = false;
+      left = __ballot_sync(0xffffffffu, entry != kNoTile);
     }
-    const int id = __shfl_sync(0xffffffffu, entry, issued & 31);
+    const int id = __shfl_sync(0xffffffffu, entry, __ffs(left) - 1);
+    left &= left - 1;
     if (lane == 0) {
       const int s = issued % kStages;
       const int from = id < 0 ? 0 : id;  // a tile that exists; its result is flagged as bad
       if (id < 0) atomicOr(a.err, B2_DEV_BAD_BLOCK);
       sh.tile[warp][s] = id;
       const uint32_t bar = smem_u32(&sh.full[warp][s]), dst = smem_u32(sh.codes[warp][s]);
-      mbar_expect_tx(bar, 2 * kTile + 32);
+      mbar_expect_tx(bar, 2 * kTile);
       bulk_load(dst, a.k_pool + static_cast<int64_t>(from) * kTile, kTile, bar, policy);
       bulk_load(dst + kTile, a.v_pool + static_cast<int64_t>(from) * kTile, kTile, bar, policy);
-      const uint32_t sc = smem_u32(sh.scales[warp][s]);
-      bulk_load(sc, a.k_scale + (from & ~3), 16, bar, policy);
-      bulk_load(sc + 16, a.v_scale + (from & ~3), 16, bar, policy);
     }
+    // (as 16-byte copies of their own the scales doubled the copies, which one
+    // thread issues at about 100 ns each)
+    scales[kStages - 1] = make_float2(__ldg(a.k_scale + max(id, 0)), __ldg(a.v_scale + max(id, 0)));
     ++issued;
   };
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) issue();
-
-  // state of the current segment: columns 2t, 2t + 1 in the lanes of thread t
-  uint32_t bq[4][2];
-  float o[4][4], m0 = kUnset, m1 = kUnset, mo0 = kUnset, mo1 = kUnset, l0 = 0.f, l1 = 0.f, f0 = 0.f, f1 = 0.f;
-  uint4 fresh[kT];  // bf16 k (lanes 16-23) and v (24-31) of the segment's new tokens
-  int b = 0, h = 0, blk = 0, nblk = 0, past = 0, ntok = 0;
-  bool ok = true;
-  if (x0 < x1) {
-    b = sequence_of(x0 / kHkv);
-    nblk = sh.prefix[b + 1] - sh.prefix[b];
-    const int r = x0 - sh.prefix[b] * kHkv;
-    h = r / nblk;
-    blk = r - h * nblk;
+  for (int s = 0; s < kStages; ++s) {
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) scales[i] = scales[i + 1];
+    issue();
   }
-  bool begin = true;      // the next tile is the segment's first in this warp
-  bool from_start = blk == 0;  // ... and the segment's first of all
-  for (int x = x0; x < x1; ++x) {
-    const int k = x - x0, s = k % kStages;
+
+  // state of the current segment: vector t + 4 u of set u in the lanes of thread t
+  constexpr int kSets = Shared::kSets;
+  uint32_t bq[4][2];
+  float o[4][4], m[kSets], mo[kSets], l[kSets], factor[kSets];
+  // head vectors of the segment's new tokens, bf16: q (lanes 0-15), k (16-23) and
+  // v (24-31), and those of the next segment on their way
+  uint4 fresh[kT], fresh_next[kT];
+  auto fetch = [&](int sb, int head) {
+    const int vec = grp < 2 ? 2 * head + grp : (grp == 2 ? kHq + head : kHq + kHkv + head);
+    const uint16_t *p = a.qkv + static_cast<int64_t>(sb) * a.tokens * a.row_stride + vec * kDim + j * 8;
+#pragma unroll
+    for (int i = 0; i < kT; ++i)
+      if (i < sh.fresh[sb]) fresh_next[i] = __ldg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
+  };
+  // the segment after (b, h): its sequence
+  auto following = [&](int sb) {
+    do ++sb; while (sb < a.batch && sh.pos[sb + 1] == sh.pos[sb]);
+    return sb;
+  };
+  if (blk >= nblk && ++h == kHkv) {  // starts behind a segment's last tile
+    h = 0;
+    b = following(b);
+  }
+  bool begin = true, from_start = false;  // the next tile is the segment's first in this warp, .. of all
+  int past = 0, ntok = 0;
+  bool ok = true;
+  if (issued > 0) {
+    if (blk >= nblk) blk = 0;
+    nblk = (sh.pos[b + 1] - sh.pos[b]) / kHkv - kSegmentCost;
+    from_start = blk == 0;
+    fetch(b, h);
+  }
+  for (int k = 0; k < issued; ++k) {
+    const int s = k % kStages;
     if (begin) {
       // queries of the segment: norm + RoPE, then f16 columns in shared memory
-      lengths(b, past, ntok);
-      const int vec = grp < 2 ? 2 * h + grp : (grp == 2 ? kHq + h : kHq + kHkv + h);
+      past = sh.past[b];
+      ntok = sh.fresh[b];
 #pragma unroll
-      for (int i = 0; i < kT; ++i)
-        if (i < ntok)
-          fresh[i] = __ldg(reinterpret_cast<const uint4 *>(
-              a.qkv + (static_cast<int64_t>(b) * a.tokens + i) * a.row_stride + vec * kDim + j * 8));
+      for (int i = 0; i < kT; ++i) fresh[i] = fresh_next[i];
+      if (sh.pos[b] + (h + 1) * (nblk + kSegmentCost) < w1)  // another segment follows: its rows are here by then
+        fetch(h + 1 < kHkv ? b : following(b), (h + 1) % kHkv);
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < kT; ++i) {
@@ -734,37 +789,38 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
         if (grp < 2) {
-          // the column's largest value at 2^8: f16 keeps all bf16 bits of values down to 2^-22 of it
+          // the query with its largest value in [2^8, 2^9)
           int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
           e = e < -100 ? -100 : e;
           const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
-          uint4 w;
-          w.x = pack_f16x2(y[0] * up, y[1] * up);
-          w.y = pack_f16x2(y[2] * up, y[3] * up);
-          w.z = pack_f16x2(y[4] * up, y[5] * up);
-          w.w = pack_f16x2(y[6] * up, y[7] * up);
-          *reinterpret_cast<uint4 *>(&sh.row[warp].q[2 * i + grp][8 * j]) = w;
-          if (j == 0) sh.factor[warp][2 * i + grp] = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
+          const int v = 2 * i + grp;
+          *reinterpret_cast<uint4 *>(&sh.row[warp].q[v][8 * j]) =
+              make_uint4(pack_f16x2(y[0] * up, y[1] * up), pack_f16x2(y[2] * up, y[3] * up),
+                         pack_f16x2(y[4] * up, y[5] * up), pack_f16x2(y[6] * up, y[7] * up));
+          if (j == 0) sh.factor[warp][v] = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
         }
       }
       __syncwarp();
-      const bool mine = g < 2 * ntok;
+      // column g holds vector g / 2 (g even) or 4 + g / 2
+      const int qv = (g >> 1) + 4 * (g & 1);
       uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
-      if (mine) {
-        const uint4 *p = reinterpret_cast<const uint4 *>(&sh.row[warp].q[g][16 * t]);
+      if (qv < 2 * ntok) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(&sh.row[warp].q[qv][16 * t]);
         w0 = p[0];
         w1 = p[1];
       }
       bq[0][0] = w0.x; bq[0][1] = w0.y; bq[1][0] = w0.z; bq[1][1] = w0.w;
       bq[2][0] = w1.x; bq[2][1] = w1.y; bq[3][0] = w1.z; bq[3][1] = w1.w;
-      f0 = t < ntok ? sh.factor[warp][2 * t] : 0.f;
-      f1 = t < ntok ? sh.factor[warp][2 * t + 1] : 0.f;
-      m0 = m1 = mo0 = mo1 = kUnset;
-      l0 = l1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+      for (int u = 0; u < kSets; ++u) {
+        factor[u] = 4 * u + t < 2 * ntok ? sh.factor[warp][4 * u + t] : 0.f;
+        m[u] = mo[u] = kUnset;
+        l[u] = 0.f;
+      }
       begin = false;
     }
     if (!mbar_wait(smem_u32(&sh.full[warp][s]), (k / kStages) & 1, a.wait_ns)) ok = false;
@@ -774,7 +830,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
       break;
     }
     uint8_t *kc = sh.codes[warp][s], *vc = kc + kTile;
-    float ks = sh.scales[warp][s][h & 3], vs = sh.scales[warp][s][4 + (h & 3)];
+    float ks = scales[0].x, vs = scales[0].y;
     const int key0 = blk * kBlock;
 
     if ((a.mode & B2_STORE_KV) && key0 + kBlock > past && sh.tile[warp][s] >= 0) {
@@ -850,166 +906,163 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
       __syncwarp();
     }
 
-    // S = K . Q^T: row g of m-tile i, half u, is token 16 (g / 2) + 4 i + 2 u + g % 2
+    // S = K . Q^T: row g of m-tile i is token 16 (g / 2) + 4 i + g % 2, row g + 8
+    // the one two behind it (8 lanes of a load read two adjacent rows)
+    const int tok0 = 16 * (g >> 1) + (g & 1), tok1 = tok0 + 2;
     float c[4][4];
+    uint4 r[4][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint8_t *p = kc + (16 * (g >> 1) + 4 * i + (g & 1)) * kDim + 16 * t;
-      const uint4 r0 = *reinterpret_cast<const uint4 *>(p), r1 = *reinterpret_cast<const uint4 *>(p + 2 * kDim);
+      r[i][0] = *reinterpret_cast<const uint4 *>(kc + (tok0 + 4 * i) * kDim + 16 * t);
+      r[i][1] = *reinterpret_cast<const uint4 *>(kc + (tok1 + 4 * i) * kDim + 16 * t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
-      mma_codes(c[i], r0, r1, bq);
     }
-    // scores in log2 units against the reference m
-    const float w0 = f0 * ks, w1 = f1 * ks;
+    mma_codes(c, r, bq);
     const bool tail = key0 + kBlock > past + 1;  // some token does not see the whole tile
-    if (tail) {
-      const int lim = past + t + 1 - key0;  // token t sees rows < lim
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = 16 * (g >> 1) + 4 * i + (e & 2) + (g & 1);
-          if (tok >= lim) c[i][e] = -INFINITY;
-          else c[i][e] *= (e & 1) ? w1 : w0;
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[i][e] *= (e & 1) ? w1 : w0;
-    }
-    float top0 = c[0][0], top1 = c[0][1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      top0 = fmaxf(top0, fmaxf(c[i][0], c[i][2]));
-      top1 = fmaxf(top1, fmaxf(c[i][1], c[i][3]));
-    }
-    if (__any_sync(0xffffffffu, t < ntok && (top0 > m0 + kSlack || top1 > m1 + kSlack))) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        top0 = fmaxf(top0, __shfl_xor_sync(0xffffffffu, top0, off));
-        top1 = fmaxf(top1, __shfl_xor_sync(0xffffffffu, top1, off));
-      }
-      const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
-      l0 *= ex2(m0 - n0);
-      l1 *= ex2(m1 - n1);
-      m0 = n0;
-      m1 = n1;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[i][0] = ex2(c[i][0] - m0);
-      c[i][1] = ex2(c[i][1] - m1);
-      c[i][2] = ex2(c[i][2] - m0);
-      c[i][3] = ex2(c[i][3] - m1);
-      l0 += c[i][0] + c[i][2];
-      l1 += c[i][1] + c[i][3];
-    }
-    // p * v scale against the reference mo (mantissa and exponent of the scale apart)
-    const uint32_t vbits = __float_as_uint(vs);
+    const uint32_t vbits = __float_as_uint(vs);  // mantissa and exponent of the v scale apart
     const float vmant = __uint_as_float((vbits & 0x007fffffu) | 0x3f800000u);
     const float vexp = static_cast<float>(static_cast<int>(vbits >> 23) - 127);
-    float g0 = vmant * ex2(m0 - mo0 + vexp), g1 = vmant * ex2(m1 - mo1 + vexp);
-    if (__any_sync(0xffffffffu, t < ntok && (g0 > kMaxGain || g1 > kMaxGain))) {
-      float p0 = c[0][0], p1 = c[0][1];
+    float p[kSets][4][2];  // p * g of rows g and g + 8
+#pragma unroll
+    for (int u = 0; u < kSets; ++u) {
+      const bool used = 4 * u + t < 2 * ntok;
+      // scores in log2 units of rows g (x) and g + 8 (y)
+      const float w = factor[u] * ks;
+      float x[4], y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p0 = fmaxf(p0, fmaxf(c[i][0], c[i][2]));
-        p1 = fmaxf(p1, fmaxf(c[i][1], c[i][3]));
+        x[i] = c[i][u] * w;
+        y[i] = c[i][2 + u] * w;
       }
+      if (tail) {
+        const int lim = past + ((4 * u + t) >> 1) + 1 - key0;  // the vector's token sees rows < lim
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        p0 = fmaxf(p0, __shfl_xor_sync(0xffffffffu, p0, off));
-        p1 = fmaxf(p1, __shfl_xor_sync(0xffffffffu, p1, off));
+        for (int i = 0; i < 4; ++i) {
+          if (tok0 + 4 * i >= lim) x[i] = -INFINITY;
+          if (tok1 + 4 * i >= lim) y[i] = -INFINITY;
+        }
       }
-      // the largest product at 1
-      const float n0 = p0 > 0.f ? fmaxf(mo0, m0 + vexp + __log2f(p0)) : mo0;
-      const float n1 = p1 > 0.f ? fmaxf(mo1, m1 + vexp + __log2f(p1)) : mo1;
-      const float a0 = ex2(mo0 - n0), a1 = ex2(mo1 - n1);
+      float top = fmaxf(fmaxf(fmaxf(x[0], y[0]), fmaxf(x[1], y[1])), fmaxf(fmaxf(x[2], y[2]), fmaxf(x[3], y[3])));
+      if (__any_sync(0xffffffffu, used && top > m[u] + kSlack)) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float n = fmaxf(m[u], top);
+        l[u] *= ex2(m[u] - n);
+        m[u] = n;
+      }
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[i][0] *= a0;
-        o[i][1] *= a1;
-        o[i][2] *= a0;
-        o[i][3] *= a1;
+        x[i] = ex2(x[i] - m[u]);
+        y[i] = ex2(y[i] - m[u]);
+        sum += x[i] + y[i];
       }
-      mo0 = n0;
-      mo1 = n1;
-      g0 = vmant * ex2(m0 - mo0 + vexp);
-      g1 = vmant * ex2(m1 - mo1 + vexp);
+      l[u] += sum;
+      float gain = vmant * ex2(m[u] - mo[u] + vexp);
+      if (__any_sync(0xffffffffu, used && gain > kMaxGain)) {
+        float big = fmaxf(fmaxf(fmaxf(x[0], y[0]), fmaxf(x[1], y[1])), fmaxf(fmaxf(x[2], y[2]), fmaxf(x[3], y[3])));
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+        // the largest product so far at 1
+        const float n = big > 0.f ? fmaxf(mo[u], m[u] + vexp + __log2f(big * vmant)) : mo[u];
+        const float again = ex2(mo[u] - n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i][u] *= again;
+          o[i][2 + u] *= again;
+        }
+        mo[u] = n;
+        gain = vmant * ex2(m[u] - n + vexp);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[u][i][0] = x[i] * gain;
+        p[u][i][1] = y[i] * gain;
+      }
     }
-    uint32_t bp[4][2];
+    uint32_t bp[4][2];  // P^T: tokens 16 t + 4 i + {0, 1} and + {2, 3} of column g
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        bp[i][e] = transpose8x8(pack_f16x2(p[0][i][e], kSets > 1 ? p[kSets - 1][i][e] : 0.f));
+    // O^T += V^T . P^T: rows g and g + 8 of m-tile i are dims 16 i + g and 16 i + 8 + g
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      bp[i][0] = transpose8x8(pack_f16x2(c[i][0] * g0, c[i][1] * g1));
-      bp[i][1] = transpose8x8(pack_f16x2(c[i][2] * g0, c[i][3] * g1));
+      const uint8_t *row = vc + (16 * i + g) * kBlock + 16 * t;
+      r[i][0] = *reinterpret_cast<const uint4 *>(row);
+      r[i][1] = *reinterpret_cast<const uint4 *>(row + 8 * kBlock);
     }
-    // O^T += V^T . P^T: row g of m-tile i, half u, is dim 16 i + 8 u + g
-    uint4 keep = make_uint4(~0u, ~0u, ~0u, ~0u);  // codes of rows past the sequence must not meet p = 0
     if (tail) {
+      // codes of rows past the sequence must not meet p = 0
       const int n = past + ntok - key0 - 16 * t;
       auto mask = [&](int i) { return n >= 4 * i + 4 ? ~0u : (n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1u); };
-      keep = make_uint4(mask(0), mask(1), mask(2), mask(3));
-    }
+      const uint4 keep = make_uint4(mask(0), mask(1), mask(2), mask(3));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t *p = vc + (16 * i + g) * kBlock + 16 * t;
-      uint4 r0 = *reinterpret_cast<const uint4 *>(p), r1 = *reinterpret_cast<const uint4 *>(p + 8 * kBlock);
-      if (tail) {
-        r0.x &= keep.x; r0.y &= keep.y; r0.z &= keep.z; r0.w &= keep.w;
-        r1.x &= keep.x; r1.y &= keep.y; r1.z &= keep.z; r1.w &= keep.w;
-      }
-      mma_codes(o[i], r0, r1, bp);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          r[i][e].x &= keep.x;
+          r[i][e].y &= keep.y;
+          r[i][e].z &= keep.z;
+          r[i][e].w &= keep.w;
+        }
     }
+    mma_codes(o, r, bp);
     __syncwarp();
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) scales[i] = scales[i + 1];
     issue();  // the stage is read: its next tile
+    if (!looked && base + 32 < w1) {
+      entry_next = look(base + 32 + lane, false);
+      looked = true;
+    }
 
     const bool last = blk + 1 == nblk;  // of the segment
-    if (last || x + 1 == x1) {
+    if (last || k + 1 == issued) {
+      // the output in units of 2^m, as the sum; dims 16 i + g, 16 i + 8 + g
+      float s[kSets];
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+      for (int u = 0; u < kSets; ++u) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], off);
+        s[u] = ex2(mo[u] - m[u]);
       }
-      // the output in units of 2^m, as the sum
-      float s0 = ex2(mo0 - m0), s1 = ex2(mo1 - m1);
       if (last && from_start) {
-        s0 /= l0;
-        s1 /= l1;
-        if (t < ntok) {
+#pragma unroll
+        for (int u = 0; u < kSets; ++u) {
+          const int v = 4 * u + t;
+          if (v >= 2 * ntok) continue;
+          const float f = s[u] / l[u];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sh.row[warp].out[2 * t][16 * i + g] = static_cast<uint16_t>(bf16_bits(o[i][0] * s0));
-            sh.row[warp].out[2 * t + 1][16 * i + g] = static_cast<uint16_t>(bf16_bits(o[i][1] * s1));
-            sh.row[warp].out[2 * t][16 * i + 8 + g] = static_cast<uint16_t>(bf16_bits(o[i][2] * s0));
-            sh.row[warp].out[2 * t + 1][16 * i + 8 + g] = static_cast<uint16_t>(bf16_bits(o[i][3] * s1));
+            sh.row[warp].out[v][16 * i + g] = static_cast<uint16_t>(bf16_bits(o[i][u] * f));
+            sh.row[warp].out[v][16 * i + 8 + g] = static_cast<uint16_t>(bf16_bits(o[i][2 + u] * f));
           }
         }
         __syncwarp();
         for (int c8 = lane; c8 < 2 * ntok * 8; c8 += 32) {
-          const int col = c8 >> 3;
-          *reinterpret_cast<uint4 *>(a.out + ((static_cast<int64_t>(b) * a.tokens + (col >> 1)) * kHq + 2 * h + (col & 1)) * kDim +
-                                     8 * (c8 & 7)) = *reinterpret_cast<const uint4 *>(&sh.row[warp].out[col][8 * (c8 & 7)]);
+          const int v = c8 >> 3;
+          *reinterpret_cast<uint4 *>(a.out + ((static_cast<int64_t>(b) * a.tokens + (v >> 1)) * kHq + 2 * h + (v & 1)) * kDim +
+                                     8 * (c8 & 7)) = *reinterpret_cast<const uint4 *>(&sh.row[warp].out[v][8 * (c8 & 7)]);
         }
         __syncwarp();
       } else {
         // open: began before this range (head), or goes on behind it (in the ring, idle by then)
         const int which = from_start ? 1 : 0;
         State *st = which ? reinterpret_cast<State *>(sh.codes[warp][0]) : &sh.head[warp];
-        if (t < kT) {
+#pragma unroll
+        for (int u = 0; u < kSets; ++u) {
+          const int v = 4 * u + t;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            st->o[2 * t][16 * i + g] = o[i][0] * s0;
-            st->o[2 * t + 1][16 * i + g] = o[i][1] * s1;
-            st->o[2 * t][16 * i + 8 + g] = o[i][2] * s0;
-            st->o[2 * t + 1][16 * i + 8 + g] = o[i][3] * s1;
+            st->o[v][16 * i + g] = o[i][u] * s[u];
+            st->o[v][16 * i + 8 + g] = o[i][2 + u] * s[u];
           }
           if (g == 0) {
-            st->ml[2 * t][0] = m0;
-            st->ml[2 * t][1] = l0;
-            st->ml[2 * t + 1][0] = m1;
-            st->ml[2 * t + 1][1] = l1;
+            st->ml[v][0] = m[u];
+            st->ml[v][1] = l[u];
           }
         }
         if (lane == 0) sh.open[warp][which] = b * kHkv + h;
@@ -1019,10 +1072,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
         blk = -1;
         if (++h == kHkv) {
           h = 0;
-          if (x + 1 < x1) {
-            do ++b; while (sh.prefix[b + 1] == sh.prefix[b]);
-            nblk = sh.prefix[b + 1] - sh.prefix[b];
-          }
+          b = following(b);
+          if (b < a.batch) nblk = (sh.pos[b + 1] - sh.pos[b]) / kHkv - kSegmentCost;
         }
       }
     }
@@ -1037,80 +1088,81 @@ __global__ void __launch_bounds__(kStepThreads, 1) kv8_step_kernel(const StepArg
   }
   __syncthreads();
 
-  // The CTA's partial states in tile order: run r of states of one segment is
-  // merged by warp r % kWarps
-  int run = 0;
-  for (int i = 0;; ++run) {
-    while (i < 2 * kWarps && sh.open[i >> 1][i & 1] < 0) ++i;
-    if (i == 2 * kWarps) break;
-    const int seg = sh.open[i >> 1][i & 1];
-    uint32_t members = 0;
-    for (; i < 2 * kWarps; ++i) {
-      const int other = sh.open[i >> 1][i & 1];
-      if (other == seg) members |= 1u << i;
-      else if (other >= 0) break;
-    }
-    if (run % kWarps != warp) continue;
-    StateSum<kT> sum;
-    sum.clear();
-    for (uint32_t rest = members; rest; rest &= rest - 1) {
-      const int e = __ffs(rest) - 1;
-      const State *st = (e & 1) ? reinterpret_cast<const State *>(sh.codes[e >> 1][0]) : &sh.head[e >> 1];
+  // The CTA's partial states in tile order, one per lane; those of one segment
+  // are merged by one warp per new token.
+  const int mine = lane < 2 * kWarps ? sh.open[lane >> 1][lane & 1] : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, mine);
+  uint32_t todo = __ballot_sync(0xffffffffu, mine >= 0 && (same & ((1u << lane) - 1u)) == 0);
+  for (int task = 0; todo; todo &= todo - 1) {
+    const int seg = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+    const uint32_t members = __shfl_sync(0xffffffffu, same, __ffs(todo) - 1);
+    const int sb = seg / kHkv, hh = seg - sb * kHkv, stok = sh.fresh[sb];
+    for (int v = 0; v < stok; ++v, ++task) {
+      if (task % kWarps != warp) continue;
+      const int per = (sh.pos[sb + 1] - sh.pos[sb]) / kHkv;
+      // the CTAs of the segment's first and last tile: the last ones that start
+      // at or before them (CTA c starts at position c * weight / ctas)
+      const int at = sh.pos[sb] + hh * per + ((lane & 1) ? per - kSegmentCost : 1);
+      const int cta_of = static_cast<int>((static_cast<uint64_t>(at) * static_cast<uint32_t>(ctas) - 1) /
+                                          static_cast<uint32_t>(weight));
+      const int cf = __shfl_sync(0xffffffffu, cta_of, 0), cl = __shfl_sync(0xffffffffu, cta_of, 1);
+      const int vec = 2 * v + (lane >> 4), d = 4 * (lane & 15);
+      StateSum sum;
 #pragma unroll
-      for (int v = 0; v < kT; ++v) {
-        const int col = 2 * v + (lane >> 4);
-        sum.add(v, *reinterpret_cast<const float2 *>(st->ml[col]),
-                *reinterpret_cast<const float4 *>(&st->o[col][4 * (lane & 15)]));
-      }
-    }
-    const int sb = seg / kHkv, sh_head = seg - sb * kHkv;
-    const int n = sh.prefix[sb + 1] - sh.prefix[sb];
-    const int64_t first_tile = static_cast<int64_t>(sh.prefix[sb]) * kHkv + sh_head * n;
-    // the CTAs that hold tiles of the segment (CTA c starts at tile c * total / ctas)
-    const int cf = static_cast<int>(((first_tile + 1) * ctas - 1) / total);
-    const int cl = static_cast<int>(((first_tile + n) * ctas - 1) / total);
-    int spast, stok;
-    lengths(sb, spast, stok);
-    uint16_t *dst = a.out + (static_cast<int64_t>(sb) * a.tokens * kHq + 2 * sh_head) * kDim;
-    if (cf == cl) {
-      sum.write(dst, stok, lane);
-      continue;
-    }
-    // the segment's first CTA leaves its state in slot 1, the others in slot 0
-    State *slots = reinterpret_cast<State *>(a.slots);
-    const int cta = static_cast<int>(blockIdx.x);
-    sum.store(slots + 2 * cta + (cta == cf ? 1 : 0), lane);
-    __syncwarp();
-    int arrived = 0;
-    if (lane == 0) {
-      __threadfence();
-      arrived = atomicAdd(a.counters + cf, 1) == cl - cf;
-      if (arrived) __threadfence();
-    }
-    if (!__shfl_sync(0xffffffffu, arrived, 0)) continue;
-    __syncwarp();
-    sum.clear();
-    for (int c0 = cf; c0 <= cl; c0 += 8) {
-      // eight states' loads in flight together
-#pragma unroll
-      for (int v = 0; v < kT; ++v) {
-        const int col = 2 * v + (lane >> 4);
-        float2 ml[8];
-        float4 x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int c = min(c0 + e, cl);
-          const State *st = slots + 2 * c + (c == cf ? 1 : 0);
-          ml[e] = __ldcg(reinterpret_cast<const float2 *>(st->ml[col]));
-          x[e] = __ldcg(reinterpret_cast<const float4 *>(&st->o[col][4 * (lane & 15)]));
+      for (int e0 = 0; e0 < 2 * kWarps; e0 += 16) {
+        if ((members >> e0 & 0xffffu) == 0) continue;
+        auto state = [&](int e) -> const State * {
+          return (e & 1) ? reinterpret_cast<const State *>(sh.codes[e >> 1][0]) : &sh.head[e >> 1];
+        };
+        const int e = e0 + (lane & 15);
+        float2 ml = make_float2(kUnset, 0.f);
+        if (e < 2 * kWarps && (members >> e & 1)) ml = *reinterpret_cast<const float2 *>(state(e)->ml[vec]);
+        sum.group(ml);
+        for (uint32_t rest = members >> e0 & 0xffffu; rest; rest &= rest - 1) {
+          const int i = __ffs(rest) - 1;
+          sum.add(i, *reinterpret_cast<const float4 *>(&state(e0 + i)->o[vec][d]), lane);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c0 + e <= cl) sum.add(v, ml[e], x[e]);
       }
+      uint16_t *dst = a.out + ((static_cast<int64_t>(sb) * a.tokens + v) * kHq + 2 * hh) * kDim;
+      if (cf == cl) {
+        sum.write(dst, lane);
+        continue;
+      }
+      // the segment's first CTA leaves its state in slot 1, the others in slot 0
+      State *slots = reinterpret_cast<State *>(a.slots);
+      const int cta = static_cast<int>(blockIdx.x);
+      State *slot = slots + 2 * cta + (cta == cf ? 1 : 0);
+      *reinterpret_cast<float4 *>(&slot->o[vec][d]) = sum.o;
+      if (d == 0) *reinterpret_cast<float2 *>(slot->ml[vec]) = make_float2(sum.m, sum.l);
+      __syncwarp();
+      int32_t *counter = a.counters + cf * kMaxStepTokens + v;
+      int arrived = 0;
+      if (lane == 0) {
+        fence_gpu();
+        arrived = atomicAdd(counter, 1) == cl - cf;
+        if (arrived) fence_gpu();
+      }
+      if (!__shfl_sync(0xffffffffu, arrived, 0)) continue;
+      __syncwarp();
+      StateSum whole;
+      for (int c0 = cf; c0 <= cl; c0 += 16) {
+        // sixteen states' loads in flight together
+        const int c = c0 + (lane & 15);
+        float2 ml = make_float2(kUnset, 0.f);
+        if (c <= cl) ml = __ldcg(reinterpret_cast<const float2 *>((slots + 2 * c + (c == cf ? 1 : 0))->ml[vec]));
+        float4 x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int q = min(c0 + e, cl);
+          x[e] = __ldcg(reinterpret_cast<const float4 *>(&(slots + 2 * q + (q == cf ? 1 : 0))->o[vec][d]));
+        }
+        whole.group(ml);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) whole.add(e, x[e], lane);  // factor 0 past the last state
+      }
+      whole.write(dst, lane);
+      if (lane == 0) *counter = 0;
     }
-    sum.write(dst, stok, lane);
-    if (lane == 0) a.counters[cf] = 0;
   }
 }
 
@@ -1140,16 +1192,17 @@ int sm_count() {
   return count[dev];
 }
 
-constexpr int64_t kCounterBytes = kMaxCtas * 4;
+constexpr int64_t kCounterBytes = kMaxCtas * kMaxStepTokens * 4;
 constexpr int64_t kWorkspaceBytes = kCounterBytes + 2 * kMaxCtas * static_cast<int64_t>(sizeof(StepShared<kMaxStepTokens>::State));
 
 template <int kT>
 int launch_step(StepArgs a, cudaStream_t st) {
   if (!step_ready<kT>()) return fail(B2_ERR_CUDA, "cannot set the step kernel's shared memory size");
   // launches of at most kMaxSeqs sequences whose tiles an int32 counts
-  const int64_t most = ((int64_t(1) << 28) - 1) / a.max_blocks;
+  const int64_t most = ((int64_t(1) << 28) - 1) / (a.max_blocks + kSegmentCost);
   const int per = static_cast<int>(most < kMaxSeqs ? (most < 1 ? 1 : most) : kMaxSeqs);
   const int batch = a.batch;
+  constexpr int kWarps = step_warps<kT>();
   for (int b0 = 0; b0 < batch; b0 += per) {
     a.batch = batch - b0 < per ? batch - b0 : per;
     const int64_t tiles = static_cast<int64_t>(a.batch) * a.max_blocks * kHkv;
@@ -1158,7 +1211,7 @@ int launch_step(StepArgs a, cudaStream_t st) {
     if (ctas > kMaxCtas) ctas = kMaxCtas;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(ctas));
-    cfg.blockDim = dim3(kStepThreads);
+    cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = sizeof(StepShared<kT>) + 128;
     cfg.stream = st;
     cudaLaunchAttribute pdl[1];
@@ -1280,7 +1333,7 @@ extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32
              scale * 1.4426950408889634f, mode, out, static_cast<int32_t *>(workspace),
              reinterpret_cast<float *>(static_cast<char *>(workspace) + kCounterBytes), dev_err, b2_wait_limit_ns()};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return tokens == 1 ? launch_step<1>(a, st) : launch_step<kMaxStepTokens>(a, st);
+  return tokens <= 2 ? launch_step<2>(a, st) : launch_step<kMaxStepTokens>(a, st);
 }
 
 extern "C" int b2_kv8_prefill_attn(const uint16_t *q, int64_t q_stride, int32_t rows, const int32_t *row_start,
