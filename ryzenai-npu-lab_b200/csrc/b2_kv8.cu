@@ -3,7 +3,8 @@
 //
 //   kv8_append_kernel  q/k norm + RoPE and the quantised append of new tokens
 //   kv8_step_kernel    a whole decode step: append and split attention
-//   kv8_attn_kernel    causal attention of a prompt chunk over the cache
+//   kv8_prefill_kernel causal attention of a prompt chunk over the cache (tcgen05)
+//   kv8_merge_kernel   merge of a prompt tile's keys split over CTAs
 
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -276,120 +277,6 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
       }
     }
   }
-}
-
-// ------------------------------------------------------------------ attention
-
-struct AttnArgs {
-  const uint16_t *q;
-  int64_t q_stride;
-  int rows;
-  const int32_t *row_start, *past_lens, *chunk_lens;
-  int tokens;
-  const int32_t *block_tables;
-  int max_blocks;
-  const uint8_t *k_pool, *v_pool;
-  const float *k_scale, *v_scale;
-  int num_blocks, batch;
-  float scale_log2;
-  uint16_t *out;
-  int32_t *err;
-};
-
-// One CTA per (new token, KV head): its 4 warps take the 64-token blocks in
-// turn, each with its own running maximum and sum (log2 units), and are merged
-// at the end.  Lane l scores tokens l and l + 32 and sums dims l and l + 32.
-__global__ void __launch_bounds__(128) kv8_attn_kernel(const AttnArgs a) {
-  __shared__ float qs[2][kDim];
-  __shared__ float ps[4][2][kBlock];
-  __shared__ float red[4][2][2 + kDim];
-  const int b = blockIdx.x / a.tokens, t = blockIdx.x - b * a.tokens, h = blockIdx.y;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
-  if (t >= chunk) return;
-  const int past = a.past_lens[b];
-  const int64_t row = (a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens) + t;
-  if (past < 0 || chunk > a.tokens || static_cast<int64_t>(past) + chunk > static_cast<int64_t>(a.max_blocks) * kBlock ||
-      row < 0 || row >= a.rows) {
-    if (threadIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
-    return;
-  }
-  if (threadIdx.x < 2 * kDim) {
-    const int g = threadIdx.x >> 6, d = threadIdx.x & 63;
-    qs[g][d] = __uint_as_float(static_cast<uint32_t>(a.q[row * a.q_stride + (2 * h + g) * kDim + d]) << 16) * a.scale_log2;
-  }
-  __syncthreads();
-  const int n = past + t + 1, nblk = (n + kBlock - 1) / kBlock;
-  float m[2] = {-1.0e30f, -1.0e30f}, l[2] = {0.f, 0.f}, o[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-  for (int i = warp; i < nblk; i += 4) {
-    const int blk = a.block_tables[static_cast<int64_t>(b) * a.max_blocks + i];
-    if (blk < 0 || blk >= a.num_blocks) {
-      if (lane == 0) atomicOr(a.err, B2_DEV_BAD_BLOCK);
-      continue;
-    }
-    const int64_t si = static_cast<int64_t>(blk) * kHkv + h;
-    const uint8_t *k = a.k_pool + si * kTile, *v = a.v_pool + si * kTile;
-    const float ks = a.k_scale[si], vs = a.v_scale[si];
-    const int valid = min(kBlock, n - i * kBlock);
-    float s[2][2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int tok = lane + 32 * half;
-      float s0 = 0.f, s1 = 0.f;
-      for (int d = 0; d < kDim; d += 2) {
-        const float2 x = from_e4m3x2(*reinterpret_cast<const uint16_t *>(k + tok * kDim + d));
-        s0 += x.x * qs[0][d] + x.y * qs[0][d + 1];
-        s1 += x.x * qs[1][d] + x.y * qs[1][d + 1];
-      }
-      s[half][0] = tok < valid ? s0 * ks : -INFINITY;
-      s[half][1] = tok < valid ? s1 * ks : -INFINITY;
-    }
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const float mn = fmaxf(m[g], warp_max(fmaxf(s[0][g], s[1][g])));
-      const float c = ex2(m[g] - mn);
-      m[g] = mn;
-      const float p0 = ex2(s[0][g] - mn), p1 = ex2(s[1][g] - mn);
-      l[g] = l[g] * c + p0 + p1;
-      o[g][0] *= c;
-      o[g][1] *= c;
-      ps[warp][g][lane] = p0 * vs;
-      ps[warp][g][lane + 32] = p1 * vs;
-    }
-    __syncwarp();
-    for (int tok = 0; tok < valid; ++tok) {
-      const float v0 = from_e4m3x2(v[lane * kBlock + tok]).x, v1 = from_e4m3x2(v[(lane + 32) * kBlock + tok]).x;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        o[g][0] = fmaf(ps[warp][g][tok], v0, o[g][0]);
-        o[g][1] = fmaf(ps[warp][g][tok], v1, o[g][1]);
-      }
-    }
-    __syncwarp();
-  }
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], off);
-    red[warp][g][2 + lane] = o[g][0];
-    red[warp][g][2 + lane + 32] = o[g][1];
-    if (lane == 0) {
-      red[warp][g][0] = m[g];
-      red[warp][g][1] = l[g];
-    }
-  }
-  __syncthreads();
-  const int g = threadIdx.x >> 6, d = threadIdx.x & 63;
-  float M = -1.0e30f, L = 0.f, O = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, red[w][g][0]);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float c = ex2(red[w][g][0] - M);
-    L = fmaf(red[w][g][1], c, L);
-    O = fmaf(red[w][g][2 + d], c, O);
-  }
-  a.out[(row * kHq + 2 * h + g) * kDim + d] = static_cast<uint16_t>(bf16_bits(O / L));
 }
 
 // ------------------------------------------------------------------ decode step
@@ -1193,7 +1080,7 @@ int sm_count() {
 }
 
 constexpr int64_t kCounterBytes = kMaxCtas * kMaxStepTokens * 4;
-constexpr int64_t kWorkspaceBytes = kCounterBytes + 2 * kMaxCtas * static_cast<int64_t>(sizeof(StepShared<kMaxStepTokens>::State));
+constexpr int64_t kStepBytes = kCounterBytes + 2 * kMaxCtas * static_cast<int64_t>(sizeof(StepShared<kMaxStepTokens>::State));
 
 template <int kT>
 int launch_step(StepArgs a, cudaStream_t st) {
@@ -1231,6 +1118,558 @@ int launch_step(StepArgs a, cudaStream_t st) {
   return b2_clear_error();
 }
 
+// ------------------------------------------------------------------ prompt chunks
+
+// Attention of a chunk of new tokens per sequence, appended before, on the
+// tcgen05 tensor cores.  One CTA per (64-token query tile, KV head, sequence)
+// holds 128 query rows (64 tokens x the pair of heads) and walks the
+// sequence's 64-token blocks:
+//   S_j[128 x 64]  = Q[128 x 64] . K_j^T     into tensor memory, f16 operands
+//   O[128 x 64]   += P_j[128 x 64] . V_j     P_j as the A operand from tensor memory
+// Warp roles: warps 0-3 the online softmax (thread = query row = TMEM lane),
+// warp 4 issues the products, warps 5 and 6 bring K and V: each copies its 4 KiB
+// tiles of codes ahead (cp.async.bulk), converts them to f16 (exact) and stores
+// them as 128-byte-swizzled operands.  V is stored dim-major, so both B operands
+// are K-major.  S and P are double-buffered, as the operands' rings are, so
+// conversion, products and softmax of different blocks overlap.
+//
+// The scales never touch the operands: a row's scores are S * (q factor * k
+// scale), and P is p * g with g = v scale * 2^(m - mo), the references m (of
+// the sum) and mo (of the output, moved when the block's largest product
+// exceeds it by kMaxGain) as in the decode step; only moving mo needs the
+// output rescaled in tensor memory.
+//
+// Few long sequences leave most SMs idle: then the blocks of a tile are split
+// over several CTAs, whose states go through the workspace to kv8_merge_kernel,
+// launched behind as a programmatic dependent.
+constexpr int kPfStages = 3;                 // f16 operand stages of K and of V
+constexpr int kPfRaw = 4;                    // stages of codes
+constexpr int kPfThreads = 7 * 32;
+constexpr int kPfTmemCols = 256;             // S at columns 0 and 64, O at 128, P at 192 and 224
+constexpr int kPfOperand = kBlock * kDim * 2;
+constexpr int kPfMaxSplit = 32;
+constexpr int kPfMaxParts = 320;             // CTAs of a split launch
+constexpr uint32_t kPfIdesc = (1u << 4) | (8u << 17) | (8u << 24);  // f32 <- f16, M 128, N 64, both K-major
+
+struct __align__(16) PrefillTail {
+  uint64_t raw[2][kPfRaw];       // codes landed (K, V)
+  uint64_t full[2][kPfStages];   // operand written by its converter warp
+  uint64_t empty[2][kPfStages];  // operand read by its product (commit)
+  uint64_t sbar[2];              // S_j computed (commit)
+  uint64_t sfree[2];             // S_j read by the softmax threads
+  uint64_t pready[2];            // P_j written by the softmax threads
+  uint64_t pfree[2];             // P_j read by its product (commit)
+  uint64_t pvbar;                // P_j . V_j accumulated (commit per block)
+  uint64_t obar;                 // every product done (one commit)
+  uint32_t tmem;
+  int abort;
+};
+constexpr int kPfSmem = 1024 + 2 * kPfOperand + 2 * kPfStages * kPfOperand + 2 * kPfRaw * kTile + (int)sizeof(PrefillTail);
+
+struct PrefillState {  // unnormalised output and (m, l) of a query tile's rows over one CTA's blocks
+  float o[2 * kBlock][kDim];
+  float ml[2 * kBlock][2];
+};
+
+struct PrefillArgs {
+  const uint16_t *q;
+  int64_t q_stride;
+  int rows;
+  const int32_t *row_start, *past_lens, *chunk_lens;
+  int tokens;
+  const int32_t *block_tables;
+  int max_blocks;
+  const uint8_t *k_pool, *v_pool;
+  const float *k_scale, *v_scale;
+  int num_blocks;
+  float scale_log2;
+  uint16_t *out;
+  int nsplit;
+  PrefillState *parts;   // [query tile][nsplit]
+  int32_t *err;
+  uint64_t wait_ns;
+};
+
+// Query tile t0 of sequence b: its first row, tokens, blocks, and the blocks of
+// one of its parts.  False: nothing there (or lengths that do not fit, flagged).
+struct PrefillTile {
+  int past, rows, blocks, per, parts;
+  int64_t row;
+};
+__device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0, bool report, PrefillTile &t) {
+  const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
+  if (t0 >= chunk) return false;
+  t.past = a.past_lens[b];
+  t.row = a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens;
+  if (t.past < 0 || chunk > a.tokens || static_cast<int64_t>(t.past) + chunk > static_cast<int64_t>(a.max_blocks) * kBlock ||
+      t.row < 0 || t.row + chunk > a.rows) {
+    if (report) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+    return false;
+  }
+  t.row += t0;
+  t.rows = min(kBlock, chunk - t0);
+  t.blocks = (t.past + t0 + t.rows - 1) / kBlock + 1;
+  t.per = (t.blocks + a.nsplit - 1) / a.nsplit;
+  t.parts = (t.blocks + t.per - 1) / t.per;
+  return true;
+}
+
+__global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const PrefillArgs a) {
+  const int h = blockIdx.y;
+  const int b = static_cast<int>(blockIdx.z) / a.nsplit, split = static_cast<int>(blockIdx.z) - b * a.nsplit;
+  // the last tiles see the most keys: they start first
+  const int tile = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x), t0 = tile * kBlock;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  PrefillTile pt;
+  if (!prefill_tile(a, b, t0, tid == 0, pt) || split >= pt.parts) return;
+  const int past = pt.past, rows_t = pt.rows, last_key = past + t0 + rows_t - 1;
+  const int64_t row0 = pt.row;
+  // this CTA's blocks [j0, j0 + nblk)
+  const int j0 = split * pt.per, nblk = min(pt.per, pt.blocks - j0);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *ring = sq + 2 * kPfOperand;                   // K stages, then V stages
+  uint8_t *raw = ring + 2 * kPfStages * kPfOperand;      // codes of K, then of V
+  PrefillTail *tail = reinterpret_cast<PrefillTail *>(raw + 2 * kPfRaw * kTile);
+
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+#pragma unroll
+      for (int s = 0; s < kPfRaw; ++s) mbar_init(smem_u32(&tail->raw[w][s]), 1);
+#pragma unroll
+      for (int s = 0; s < kPfStages; ++s) {
+        mbar_init(smem_u32(&tail->full[w][s]), 32);
+        mbar_init(smem_u32(&tail->empty[w][s]), 1);
+      }
+      mbar_init(smem_u32(&tail->sbar[w]), 1);
+      mbar_init(smem_u32(&tail->sfree[w]), 128);
+      mbar_init(smem_u32(&tail->pready[w]), 128);
+      mbar_init(smem_u32(&tail->pfree[w]), 1);
+    }
+    mbar_init(smem_u32(&tail->pvbar), 1);
+    mbar_init(smem_u32(&tail->obar), 1);
+    tail->abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
+                 "n"(kPfTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // query rows: row r = (head of the pair) * 64 + token, its largest value at 2^8 in f16
+  float factor = 0.f;
+  if (tid < 2 * kBlock) {
+    const int hl = tid >> 6, t = tid & 63;
+    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (row0 + t) * a.q_stride + (2 * h + hl) * kDim);
+    uint4 w[8];
+    float big = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      w[c] = t < rows_t ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+      float y[8];
+      unpack8(w[c], y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e]));
+    }
+    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+    e = e < -100 ? -100 : e;
+    const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
+    factor = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      float y[8];
+      unpack8(w[c], y);
+      *reinterpret_cast<uint4 *>(sq + tid * 128 + ((c ^ (tid & 7)) << 4)) =
+          make_uint4(pack_f16x2(y[0] * up, y[1] * up), pack_f16x2(y[2] * up, y[3] * up),
+                     pack_f16x2(y[4] * up, y[5] * up), pack_f16x2(y[6] * up, y[7] * up));
+    }
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = tail->tmem;
+
+  if (warp >= 5) {
+    // ---------------- K (warp 5) and V (warp 6): codes in, f16 operands out
+    const int which = warp - 5;
+    const uint8_t *pool = which ? a.v_pool : a.k_pool;
+    uint8_t *codes = raw + which * kPfRaw * kTile, *operand = ring + which * kPfStages * kPfOperand;
+    const int32_t *table = a.block_tables + static_cast<int64_t>(b) * a.max_blocks + j0;
+    const uint64_t policy = evict_first_policy();
+    int entry = lane < nblk ? table[lane] : 0, entry_next = 32 + lane < nblk ? table[32 + lane] : 0;
+    int issued = 0;
+    auto issue = [&]() {
+      if (issued >= nblk) return;
+      if (issued > 0 && (issued & 31) == 0) {
+        entry = entry_next;
+        entry_next = issued + 32 + lane < nblk ? table[issued + 32 + lane] : 0;
+      }
+      int blk = __shfl_sync(0xffffffffu, entry, issued & 31);
+      if (blk < 0 || blk >= a.num_blocks) {
+        if (lane == 0 && which == 0) atomicOr(a.err, B2_DEV_BAD_BLOCK);
+        blk = 0;  // read a valid tile instead; the result is flagged as bad
+      }
+      const int64_t id = static_cast<int64_t>(blk) * kHkv + h;
+      const int s = issued % kPfRaw;
+      if (lane == 0) {
+        const uint32_t bar = smem_u32(&tail->raw[which][s]);
+        mbar_expect_tx(bar, kTile);
+        bulk_load(smem_u32(codes + s * kTile), pool + id * kTile, kTile, bar, policy);
+      }
+      ++issued;
+    };
+    for (int s = 0; s < kPfRaw; ++s) issue();
+    for (int j = 0; j < nblk; ++j) {
+      const int s = j % kPfStages, rs = j % kPfRaw;
+      bool got = mbar_wait(smem_u32(&tail->raw[which][rs]), (j / kPfRaw) & 1, a.wait_ns);
+      uint4 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint4 *>(codes + rs * kTile + (32 * i + lane) * 16);
+      __syncwarp();
+      issue();
+      if (j >= kPfStages) got = got && mbar_wait(smem_u32(&tail->empty[which][s]), ((j / kPfStages) - 1) & 1, a.wait_ns);
+      if (__any_sync(0xffffffffu, !got || tail->abort)) {
+        if (lane == 0 && !tail->abort) atomicOr(a.err, B2_DEV_TIMEOUT);
+        tail->abort = 1;
+        break;
+      }
+      if (which && (j0 + j) * kBlock + kBlock - 1 > last_key) {
+        // tokens past the tile's last key may hold anything (even NaN): p = 0 must not meet them
+        const int n = last_key + 1 - (j0 + j) * kBlock - 16 * (lane & 3);
+        auto mask = [&](int i) { return n >= 4 * i + 4 ? ~0u : (n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1u); };
+        const uint4 keep = make_uint4(mask(0), mask(1), mask(2), mask(3));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          w[i].x &= keep.x;
+          w[i].y &= keep.y;
+          w[i].z &= keep.z;
+          w[i].w &= keep.w;
+        }
+      }
+      // piece c = 32 i + lane is 16 codes of row c / 4 (token or dim): two 16-byte pieces of f16
+      uint8_t *dst = operand + s * kPfOperand;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 8 * i + (lane >> 2), c = 2 * (lane & 3);
+        uint4 lo, hi;
+        codes_f16(w[i].x, lo.x, lo.y);
+        codes_f16(w[i].y, lo.z, lo.w);
+        codes_f16(w[i].z, hi.x, hi.y);
+        codes_f16(w[i].w, hi.z, hi.w);
+        *reinterpret_cast<uint4 *>(dst + row * 128 + ((c ^ (row & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4 *>(dst + row * 128 + (((c + 1) ^ (row & 7)) << 4)) = hi;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(smem_u32(&tail->full[which][s]));
+    }
+    // leave no copy in flight behind
+    for (int s = 0; s < kPfRaw && s < issued; ++s) {
+      const int k = s + kPfRaw * ((issued - 1 - s) / kPfRaw);
+      if (!mbar_wait(smem_u32(&tail->raw[which][s]), (k / kPfRaw) & 1, kDrainNs) && lane == 0) atomicOr(a.err, B2_DEV_TIMEOUT);
+    }
+  } else if (warp == 4) {
+    // ---------------- products: S_0, S_1, then per block P_j . V_j and S_{j+2}
+    if (lane == 0) {
+      auto issue_s = [&](int j) -> bool {
+        const int s = j % kPfStages;
+        if (!mbar_wait(smem_u32(&tail->full[0][s]), (j / kPfStages) & 1, a.wait_ns)) return false;
+        if (j >= 2 && !mbar_wait(smem_u32(&tail->sfree[j & 1]), ((j >> 1) - 1) & 1, a.wait_ns)) return false;
+        tmem_fence_after();
+        const uint32_t kt = smem_u32(ring + s * kPfOperand);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma_f16(tmem + 64 * (j & 1), umma_desc(smem_u32(sq) + 32 * ks, 16), umma_desc(kt + 32 * ks, 16), kPfIdesc, ks > 0);
+        umma_commit(smem_u32(&tail->sbar[j & 1]));
+        umma_commit(smem_u32(&tail->empty[0][s]));
+        return true;
+      };
+      bool ok = issue_s(0) && (nblk < 2 || issue_s(1));
+      for (int j = 0; ok && j < nblk; ++j) {
+        const int s = j % kPfStages;
+        if (!mbar_wait(smem_u32(&tail->pready[j & 1]), (j >> 1) & 1, a.wait_ns) || tail->abort ||
+            !mbar_wait(smem_u32(&tail->full[1][s]), (j / kPfStages) & 1, a.wait_ns)) {
+          ok = false;
+          break;
+        }
+        tmem_fence_after();
+        const uint32_t vt = smem_u32(ring + (kPfStages + s) * kPfOperand);
+        const uint32_t pt = tmem + 192 + 32 * (j & 1);  // 16 tokens per step = 8 columns
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          umma_f16_ta(tmem + 128, pt + 8 * ks, umma_desc(vt + 32 * ks, 16), kPfIdesc, (j > 0 || ks > 0) ? 1u : 0u);
+        umma_commit(smem_u32(&tail->pvbar));
+        umma_commit(smem_u32(&tail->pfree[j & 1]));
+        umma_commit(smem_u32(&tail->empty[1][s]));
+        if (j + 2 < nblk) ok = issue_s(j + 2);
+      }
+      if (!ok) {
+        if (!tail->abort) atomicOr(a.err, B2_DEV_TIMEOUT);
+        tail->abort = 1;
+      }
+      // one commit behind the last product: its phase says that all are done
+      umma_commit(smem_u32(&tail->obar));
+      if (!mbar_wait(smem_u32(&tail->obar), 0, kDrainNs)) atomicOr(a.err, B2_DEV_TIMEOUT);
+    }
+  } else {
+    // ---------------- softmax: thread = query row = TMEM lane
+    const int hl = tid >> 6, t = tid & 63;
+    const bool row_ok = t < rows_t;
+    const int qpos = past + t0 + t;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(32 * warp) << 16);
+    float m = kUnset, mo = kUnset, l = 0.f;
+    bool ok = true;
+    // decided for the whole warp: the tensor memory accesses are warp-collective
+    auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
+      const bool got = mbar_wait(bar, parity, a.wait_ns);
+      return !__any_sync(0xffffffffu, !got || tail->abort);
+    };
+    // a warp whose rows are all past the chunk keeps step with the barriers only
+    const bool active = __any_sync(0xffffffffu, row_ok);
+    // scales of 32 blocks, one per lane; the next 32 on their way
+    const int32_t *table = a.block_tables + static_cast<int64_t>(b) * a.max_blocks + j0;
+    auto pool_tile = [&](int j) -> int64_t {
+      const int blk = j < nblk ? table[j] : 0;
+      return static_cast<int64_t>(blk < 0 || blk >= a.num_blocks ? 0 : blk) * kHkv + h;
+    };
+    int64_t id = pool_tile(lane);
+    float2 scale = make_float2(__ldg(a.k_scale + id), __ldg(a.v_scale + id)), scale_next = scale;
+    for (int j = 0; j < nblk; ++j) {
+      if (!warp_wait(smem_u32(&tail->sbar[j & 1]), (j >> 1) & 1)) {
+        ok = false;
+        break;
+      }
+      if (!active) {
+        mbar_arrive(smem_u32(&tail->sfree[j & 1]));
+        if (j >= 2 && !warp_wait(smem_u32(&tail->pfree[j & 1]), ((j >> 1) - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive(smem_u32(&tail->pready[j & 1]));
+        continue;
+      }
+      tmem_fence_after();
+      if (j > 0 && (j & 31) == 0) scale = scale_next;
+      if ((j & 31) == 8) id = pool_tile((j & ~31) + 32 + lane);
+      if ((j & 31) == 16) scale_next = make_float2(__ldg(a.k_scale + id), __ldg(a.v_scale + id));
+      const float ks = __shfl_sync(0xffffffffu, scale.x, j & 31), vs = __shfl_sync(0xffffffffu, scale.y, j & 31);
+      float sc[64];
+      tmem_ld64(trow + 64 * (j & 1), sc);
+      tmem_fence_before();
+      mbar_arrive(smem_u32(&tail->sfree[j & 1]));  // S_j is in registers
+      const int key0 = (j0 + j) * kBlock;
+      const int lim = row_ok ? qpos - key0 : -1;  // tokens c <= lim are visible
+      if (__any_sync(0xffffffffu, lim < kBlock - 1)) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) sc[c] = c <= lim ? sc[c] : -INFINITY;
+      }
+      float bm8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bm8[e] = sc[e];
+#pragma unroll
+      for (int c = 8; c < 64; ++c) bm8[c & 7] = fmaxf(bm8[c & 7], sc[c]);
+      const float w = factor * ks;
+      const float top = fmaxf(fmaxf(fmaxf(bm8[0], bm8[1]), fmaxf(bm8[2], bm8[3])),
+                              fmaxf(fmaxf(bm8[4], bm8[5]), fmaxf(bm8[6], bm8[7]))) * w;
+      if (top > m + kSlack) {
+        l *= ex2(m - top);
+        m = top;
+      }
+      const uint32_t vbits = __float_as_uint(vs);
+      const float vmant = __uint_as_float((vbits & 0x007fffffu) | 0x3f800000u);
+      const float vexp = static_cast<float>(static_cast<int>(vbits >> 23) - 127);
+      float gain = vmant * ex2(m - mo + vexp), again = 1.f;
+      if (gain > kMaxGain) {
+        // the largest product so far at 1
+        const float n = fmaxf(mo, top + vexp + __log2f(vmant));
+        again = ex2(mo - n);
+        mo = n;
+        gain = vmant * ex2(m - mo + vexp);
+      }
+      if (__any_sync(0xffffffffu, again != 1.f && j > 0)) {
+        if (!warp_wait(smem_u32(&tail->pvbar), (j - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tmem_fence_after();
+#pragma unroll
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t r[16];
+          tmem_ld16_nowait(trow + 128 + c, r);
+          tmem_wait_ld();
+          float o16[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o16[e] = __uint_as_float(r[e]) * again;
+          tmem_st16(trow + 128 + c, o16);
+        }
+        tmem_wait_st();
+      }
+      float ps[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ps[e] = 0.f;
+      uint32_t pk[32];  // P_j of this row as f16 pairs
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float x0, x1;
+        ffma2(x0, x1, sc[c], sc[c + 1], w, w, -m, -m);
+        x0 = ex2(x0);
+        x1 = ex2(x1);
+        const int e = c & 7;
+        fadd2(ps[e], ps[e + 1], ps[e], ps[e + 1], x0, x1);
+        pk[c >> 1] = pack_f16x2(x0 * gain, x1 * gain);
+      }
+      l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+      // into buffer j % 2 once the product that read it is done
+      if (j >= 2 && !warp_wait(smem_u32(&tail->pfree[j & 1]), ((j >> 1) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      tmem_st32(trow + 192 + 32 * (j & 1), pk);
+      tmem_wait_st();
+      tmem_fence_before();
+      mbar_arrive(smem_u32(&tail->pready[j & 1]));
+    }
+    if (!ok) {
+      if (!tail->abort) atomicOr(a.err, B2_DEV_TIMEOUT);
+      tail->abort = 1;
+    } else if (warp_wait(smem_u32(&tail->obar), 0)) {
+      tmem_fence_after();
+      float o[64];
+      tmem_ld64(trow + 128, o);
+      const float unit = ex2(mo - m);  // the output in units of 2^m, as the sum
+      if (tail->abort) {
+      } else if (pt.parts > 1) {
+        PrefillState *st = a.parts + ((static_cast<int64_t>(b) * gridDim.x + tile) * kHkv + h) * a.nsplit + split;
+        float4 *dst = reinterpret_cast<float4 *>(st->o[tid]);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4)
+          dst[c >> 2] = make_float4(o[c] * unit, o[c + 1] * unit, o[c + 2] * unit, o[c + 3] * unit);
+        *reinterpret_cast<float2 *>(st->ml[tid]) = make_float2(m, l);
+      } else if (row_ok) {
+        const float inv = unit / l;
+        uint4 *dst = reinterpret_cast<uint4 *>(a.out + ((row0 + t) * kHq + 2 * h + hl) * kDim);
+#pragma unroll
+        for (int c = 0; c < 64; c += 8) {
+          float o8[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o8[e] = o[c + e] * inv;
+          dst[c >> 3] = pack8(o8);
+        }
+      }
+    } else {
+      atomicOr(a.err, B2_DEV_TIMEOUT);
+      tail->abort = 1;
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tmem_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPfTmemCols));
+  }
+}
+
+// The parts of a split tile's rows: 16 threads per row, 4 dims each; grid
+// (tile and head, 8 groups of 16 rows, sequence).
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const PrefillArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tile = static_cast<int>(blockIdx.x) / kHkv, h = static_cast<int>(blockIdx.x) % kHkv, b = blockIdx.z;
+  PrefillTile pt;
+  if (!prefill_tile(a, b, tile * kBlock, false, pt) || pt.parts == 1) return;
+  const int r = static_cast<int>(blockIdx.y) * 16 + (static_cast<int>(threadIdx.x) >> 4), d = 4 * (threadIdx.x & 15);
+  const int hl = r >> 6, t = r & 63;
+  if (t >= pt.rows) return;
+  const PrefillState *st = a.parts + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * a.nsplit;
+  float m = kUnset, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < pt.parts; p0 += 8) {
+    float2 ml[8];
+    float4 x[8];
+    float n = m;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const PrefillState *q = st + min(p0 + e, pt.parts - 1);
+      ml[e] = __ldcg(reinterpret_cast<const float2 *>(q->ml[r]));
+      x[e] = __ldcg(reinterpret_cast<const float4 *>(&q->o[r][d]));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (p0 + e >= pt.parts) ml[e] = make_float2(kUnset, 0.f);
+      n = fmaxf(n, ml[e].x);
+    }
+    const float again = ex2(m - n);
+    m = n;
+    l *= again;
+    o.x *= again;
+    o.y *= again;
+    o.z *= again;
+    o.w *= again;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = p0 + e < pt.parts ? ex2(ml[e].x - n) : 0.f;
+      l = fmaf(ml[e].y, f, l);
+      o.x = fmaf(x[e].x, f, o.x);
+      o.y = fmaf(x[e].y, f, o.y);
+      o.z = fmaf(x[e].z, f, o.z);
+      o.w = fmaf(x[e].w, f, o.w);
+    }
+  }
+  const float inv = 1.0f / l;
+  *reinterpret_cast<uint2 *>(a.out + ((pt.row + t) * kHq + 2 * h + hl) * kDim + d) =
+      make_uint2(pack_bf16x2_rn(o.x * inv, o.y * inv), pack_bf16x2_rn(o.z * inv, o.w * inv));
+}
+
+// the step's counters and states, then the prompt's states
+constexpr int64_t kWorkspaceBytes = kStepBytes + kPfMaxParts * static_cast<int64_t>(sizeof(PrefillState));
+
+bool prefill_ready() {
+  static std::atomic<bool> done[128];  // the attribute is per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return false;
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kv8_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmem) != cudaSuccess)
+      return false;
+    done[dev] = true;
+  }
+  return true;
+}
+
+int launch_prefill(PrefillArgs a, int batch, int max_blocks, cudaStream_t st) {
+  if (!prefill_ready()) return fail(B2_ERR_CUDA, "cannot set the prefill kernel's shared memory size");
+  const int tiles = (a.tokens + kBlock - 1) / kBlock;
+  const int64_t ctas = static_cast<int64_t>(tiles) * kHkv * batch;
+  // Split the keys when the tiles leave SMs without a CTA: about two CTAs per
+  // SM, of at least 4 blocks each (as far as the table's width tells).
+  a.nsplit = 1;
+  const int want = 2 * sm_count() < kPfMaxParts ? 2 * sm_count() : kPfMaxParts;
+  if (ctas * 2 <= want) {
+    int64_t n = want / ctas;
+    if (n > kPfMaxSplit) n = kPfMaxSplit;
+    if (n > (max_blocks + 3) / 4) n = (max_blocks + 3) / 4;
+    if (n > 1) a.nsplit = static_cast<int>(n);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles), kHkv, static_cast<unsigned>(batch * a.nsplit));
+  cfg.blockDim = dim3(kPfThreads);
+  cfg.dynamicSmemBytes = kPfSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = pdl;
+  cfg.numAttrs = 1;
+  int rc = launched(cudaLaunchKernelEx(&cfg, kv8_prefill_kernel, a), "kv8_prefill_kernel");
+  if (rc || a.nsplit == 1) return rc;
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * kHkv), 8, static_cast<unsigned>(batch));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return launched(cudaLaunchKernelEx(&cfg, kv8_merge_kernel, a), "kv8_merge_kernel");
+}
+
 // ------------------------------------------------------------------ host checks
 
 int check_cache(const void *k_pool, const void *v_pool, const void *k_scale, const void *v_scale, int32_t num_blocks) {
@@ -1264,11 +1703,6 @@ int launch_append(const AppendArgs &a, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kWindow - 1) / kWindow);
   kv8_append_kernel<<<grid, 256, 0, st>>>(a);
   return launched(cudaSuccess, "kv8_append_kernel");
-}
-
-int launch_attn(const AttnArgs &a, cudaStream_t st) {
-  kv8_attn_kernel<<<dim3(static_cast<unsigned>(a.batch * a.tokens), kHkv), 128, 0, st>>>(a);
-  return launched(cudaSuccess, "kv8_attn_kernel");
 }
 
 }  // namespace
@@ -1356,8 +1790,10 @@ extern "C" int b2_kv8_prefill_attn(const uint16_t *q, int64_t q_stride, int32_t 
   if (!workspace || !aligned16(workspace) || workspace_bytes < kWorkspaceBytes)
     return fail(B2_ERR_ARG, "workspace must be 16-byte aligned and hold b2_kv8_workspace_bytes()");
   if (!(scale > 0.f)) return fail(B2_ERR_ARG, "scale must be positive");
-  if (static_cast<int64_t>(batch) * tokens > 0x7fffffff) return fail(B2_ERR_ARG, "batch * tokens too large");
-  AttnArgs a{q, q_stride, rows, row_start, past_lens, chunk_lens, tokens, block_tables, max_blocks_per_seq,
-             k_pool, v_pool, k_scale, v_scale, num_blocks, batch, scale * 1.4426950408889634f, out, dev_err};
-  return launch_attn(a, static_cast<cudaStream_t>(stream));
+  if ((static_cast<int64_t>(tokens) + kBlock - 1) / kBlock * kHkv > 0x7fffffff) return fail(B2_ERR_ARG, "tokens too large");
+  PrefillArgs a{q, q_stride, rows, row_start, past_lens, chunk_lens, tokens, block_tables, max_blocks_per_seq,
+                k_pool, v_pool, k_scale, v_scale, num_blocks, scale * 1.4426950408889634f, out, 1,
+                reinterpret_cast<PrefillState *>(static_cast<char *>(workspace) + kStepBytes), dev_err,
+                b2_wait_limit_ns()};
+  return launch_prefill(a, batch, max_blocks_per_seq, static_cast<cudaStream_t>(stream));
 }
