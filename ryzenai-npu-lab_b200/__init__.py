@@ -5,11 +5,13 @@ Import with importlib (the directory name is not a Python identifier):
     pkg = importlib.import_module("ryzenai-npu-lab_b200")
 
 Modules:
-  _lib         ctypes binding of libb2attn.so (include/b2_decode_attn.h)
+  _lib         ctypes binding of libb2attn.so (the headers of include/)
   build        nvcc build of libb2attn.so for sm_100a
   rope         host RoPE cos/sin tables (the reference computes them on the host)
-  paged_cache  paged BF16 KV pool, block allocator, block tables
+  paged_cache  paged KV pools (bf16, 8 bits), block allocator, block tables
+  block_tables block tables and slot maps built on the GPU
   attention    torch-facing wrappers and the PagedDecodeAttention runner
+  attention_kv8  the same over the 8-bit cache
   operators    drop-in shims with the reference's NPU operator signatures
   distributed  sequence sharding and long-context split-KV across GPUs
   lfm2_runner  whole-token LFM2.5 decode runner (one CUDA graph per token)

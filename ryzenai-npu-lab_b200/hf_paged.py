@@ -20,6 +20,10 @@ calls:
     rotated by transformers); with a chunk of tokens it runs b2_prefill_append
     + b2_prefill_attn (tcgen05 tiles, causal within the chunk).
 
+With kv8=True the cache holds K and V in 8 bits (paged_cache.PagedKVCache8):
+1 to 4 new tokens run b2_kv8_decode_step, longer chunks b2_kv8_append +
+b2_kv8_prefill_attn.
+
 Usage:
     register()
     model.set_attn_implementation("b200_paged")     # or config._attn_implementation
@@ -38,8 +42,9 @@ import threading
 import torch
 
 from . import _lib
-from .attention import D, HKV, HQ, choose_blocks_per_split, decode_step, num_splits_for, prefill
-from .paged_cache import PagedKVCache, blocks_for
+from .attention import D, HKV, HQ, MAX_STEP_TOKENS, choose_blocks_per_split, decode_step, num_splits_for, prefill
+from .attention_kv8 import decode_step_kv8, prefill_kv8, workspace_kv8
+from .paged_cache import PagedKVCache, PagedKVCache8, blocks_for
 
 NAME = "b200_paged"
 _pending = threading.local()
@@ -123,7 +128,7 @@ class B200PagedCache(_DynamicCache):
     out in shuffled order)."""
 
     def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device="cuda",
-                 shuffle_seed: int | None = None, blocks_per_split: int | None = None):
+                 shuffle_seed: int | None = None, blocks_per_split: int | None = None, kv8: bool = False):
         super().__init__(config=config)
         text = config.get_text_config(decoder=True)
         if (text.num_attention_heads, text.num_key_value_heads, text.hidden_size // text.num_attention_heads) != \
@@ -134,8 +139,10 @@ class B200PagedCache(_DynamicCache):
         self.capacity = max_cache_len
         att_layers = [i for i, t in enumerate(text.layer_types) if t == "full_attention"]
         per_seq = blocks_for(max_cache_len)
-        self.pool = PagedKVCache(max_batch_size * per_seq, max_cache_len, num_layers=len(att_layers),
-                                 device=self.device, shuffle_seed=shuffle_seed)
+        self.kv8 = kv8
+        self.pool = (PagedKVCache8 if kv8 else PagedKVCache)(
+            max_batch_size * per_seq, max_cache_len, num_layers=len(att_layers), device=self.device,
+            shuffle_seed=shuffle_seed)
         for _ in range(max_batch_size):
             self.pool.add_sequence(0, capacity=max_cache_len)
         self.tables = self.pool.block_tables()
@@ -146,6 +153,7 @@ class B200PagedCache(_DynamicCache):
         self.bps = blocks_per_split
         splits = num_splits_for(self.tables.shape[1], blocks_per_split)
         dev = self.device
+        self.workspace = workspace_kv8(dev) if kv8 else None
         self.part_ml = torch.empty(max_batch_size * splits * HQ * 2, dtype=torch.float32, device=dev)
         self.part_o = torch.empty(max_batch_size * splits * HQ * D, dtype=torch.float32, device=dev)
         self.counters = torch.zeros(2 + HKV * max_batch_size, dtype=torch.int32, device=dev)
@@ -173,6 +181,8 @@ class B200PagedCache(_DynamicCache):
         if word:
             self.dev_err.zero_()
             self.counters.zero_()
+            if self.kv8:
+                self.workspace.zero_()
             raise RuntimeError("paged attention device error: " + "; ".join(_lib.decode_dev_err(word)))
 
 
@@ -201,8 +211,14 @@ def paged_attention(module, query: torch.Tensor, key: torch.Tensor, value: torch
     # one row per token: [q 16x64 | k 8x64 | v 8x64], the layout the kernels read
     qkv = torch.cat([query.transpose(1, 2).reshape(b, t, HQ * D), key.transpose(1, 2).reshape(b, t, HKV * D),
                      value.transpose(1, 2).reshape(b, t, HKV * D)], dim=-1).to(torch.bfloat16)
-    kp, vp = cache.pool.pool(layer.att)
     past_lens = cache._past_lens(past)
+    if cache.kv8:
+        out = torch.empty(b, t, HQ, D, dtype=torch.bfloat16, device=query.device)
+        call = decode_step_kv8 if t <= MAX_STEP_TOKENS else prefill_kv8
+        call(qkv.contiguous(), past_lens, block_tables=cache.tables, out=out, workspace=cache.workspace,
+             dev_err=cache.dev_err, mode=_lib.B2_STORE_KV, scale=scale, **cache.pool.kv8(layer.att))
+        return out, None
+    kp, vp = cache.pool.pool(layer.att)
     if t == 1:
         out = torch.empty(b, 1, HQ, D, dtype=torch.bfloat16, device=query.device)
         decode_step(qkv[:, 0], past_lens, k_pool=kp, v_pool=vp, block_tables=cache.tables,

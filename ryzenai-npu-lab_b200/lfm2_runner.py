@@ -24,6 +24,12 @@ Lfm2ShortConv.slow_forward 356-387, Lfm2DecoderLayer.forward 413-442,
 Lfm2Model.forward 483-538) and its cache update (cache_utils.py:771-786: the
 3-token conv state rolls by one per token).
 
+kv8=True keeps K and V in 8 bits (paged_cache.PagedKVCache8, half the cache
+bytes) with b2_kv8_decode_step in place of the bf16 step.  With pool_blocks as
+well, blocks are not reserved up front: device block tables (block_tables.py)
+take them from a pool of that many inside the captured token, so a pool smaller
+than max_batch full contexts serves sequences as they grow.
+
 Weights come from a state dict with the Hugging Face parameter names
 (model.layers.{i}.self_attn.q_proj.weight, ...), e.g. a random-init model.
 """
@@ -35,7 +41,9 @@ import torch
 
 from . import _lib, block
 from .attention import PagedDecodeAttention
-from .paged_cache import PagedKVCache, blocks_for
+from .attention_kv8 import PagedDecodeAttentionKV8, workspace_kv8
+from .block_tables import DeviceBlockTables
+from .paged_cache import PagedKVCache, PagedKVCache8, blocks_for
 
 LFM25_LAYER_TYPES = ("conv", "conv", "attention", "conv", "attention", "conv", "attention", "conv",
                      "attention", "conv", "attention", "conv", "attention", "conv")   # lfm25_x8.py:55-57
@@ -74,7 +82,10 @@ class LFM2DecodeRunner:
 
     def __init__(self, state_dict: dict, config: LFM2Config = LFM2Config(), *, max_batch: int,
                  max_context: int, device: torch.device | str = "cuda", use_graph: bool = True,
-                 blocks_per_split: int | None = None, fused_glue: bool = True, own_gemm: bool = False):
+                 blocks_per_split: int | None = None, fused_glue: bool = True, own_gemm: bool = False,
+                 kv8: bool = False, pool_blocks: int | None = None):
+        if pool_blocks is not None and not kv8:
+            raise ValueError("pool_blocks (blocks on demand) needs kv8=True")
         self.cfg = config
         self.device = torch.device(device)
         self.max_batch = max_batch
@@ -112,17 +123,34 @@ class LFM2DecodeRunner:
 
         n_att = len(config.attention_layers)
         per_seq = blocks_for(max_context)
-        self.cache = PagedKVCache(max_batch * per_seq, max_context, num_layers=n_att, device=dev)
-        for _ in range(max_batch):
-            self.cache.add_sequence(0, capacity=max_context)
-        self.tables = self.cache.block_tables()
-        self.attn = [PagedDecodeAttention(self.cache, lw["q_gamma"], lw["k_gamma"], max_batch, max_context + 1,
-                                          eps=config.eps, blocks_per_split=blocks_per_split,
-                                          work_blocks=max_batch * per_seq)
-                     for lw in self.layers if lw["kind"] == "attention"]
+        self.kv8 = kv8
+        self.block_tables = None      # blocks on demand
+        if pool_blocks is not None:
+            self.cache = PagedKVCache8(pool_blocks, max_context, num_layers=n_att, device=dev)
+            self.block_tables = DeviceBlockTables(max_batch, pool_blocks, max_context, dev)
+            self.tables = self.block_tables.tables
+            self._new = torch.ones(max_batch, dtype=torch.int32, device=dev)
+            self._plan = self.block_tables.plan(torch.zeros_like(self._new), tokens_per_seq=1)
+            self._refused = torch.zeros(1, dtype=torch.int64, device=dev)
+        else:
+            self.cache = (PagedKVCache8 if kv8 else PagedKVCache)(max_batch * per_seq, max_context, num_layers=n_att,
+                                                                 device=dev)
+            for _ in range(max_batch):
+                self.cache.add_sequence(0, capacity=max_context)
+            self.tables = self.cache.block_tables()
+        gammas = [(lw["q_gamma"], lw["k_gamma"]) for lw in self.layers if lw["kind"] == "attention"]
+        if kv8:
+            work = workspace_kv8(dev)     # the layers' calls run in turn
+            self.attn = [PagedDecodeAttentionKV8(self.cache, gq, gk, max_batch, max_context + 1, eps=config.eps,
+                                                 workspace=work) for gq, gk in gammas]
+        else:
+            self.attn = [PagedDecodeAttention(self.cache, gq, gk, max_batch, max_context + 1, eps=config.eps,
+                                              blocks_per_split=blocks_per_split, work_blocks=max_batch * per_seq)
+                         for gq, gk in gammas]
         self.conv_state = torch.zeros(len(config.conv_layers), max_batch, config.hidden, config.conv_l,
                                       dtype=bf, device=dev)
-        self.past = torch.zeros(max_batch, dtype=torch.int32, device=dev)
+        self.past = torch.zeros(max_batch, dtype=torch.int32, device=dev) if self.block_tables is None \
+            else self.block_tables.lens
         self.seq = torch.ones(max_batch, dtype=torch.int32, device=dev)
         self.ids = torch.zeros(max_batch, dtype=torch.long, device=dev)
         self.next_ids = torch.zeros(max_batch, dtype=torch.long, device=dev)
@@ -148,10 +176,27 @@ class LFM2DecodeRunner:
 
     def _token(self) -> None:
         """One token for every sequence: ids -> logits, next_ids; advances past."""
+        if self.block_tables is not None:
+            self.block_tables.plan(self._new, tokens_per_seq=1, out=self._plan)
+            self._refused += (self._plan.granted == 0).sum()
         if self.fused_glue:
             self._token_fused()
         else:
             self._token_torch()
+
+    def _attend(self, att: int, qkv: torch.Tensor) -> torch.Tensor:
+        """Context [B, 16, 64] of attention layer `att` for the new tokens' projections."""
+        if not self.kv8:
+            return self.attn[att].step(att, qkv, self.past, self.seq, self.tables)
+        granted = None if self.block_tables is None else self._plan.granted
+        return self.attn[att].step(att, qkv, self.past, self.tables, chunk_lens=granted)
+
+    def _advance(self) -> None:
+        """Count the token as cached (where its sequence got a block)."""
+        if self.block_tables is None:
+            self.past.add_(1)
+        else:
+            self.block_tables.advance(self._plan)
 
     def _mm(self, a: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> None:
         """out = a @ w.T: b2_gemm, or cuBLAS with own_gemm=False."""
@@ -174,7 +219,7 @@ class LFM2DecodeRunner:
         for i, lw in enumerate(self.layers):
             if lw["kind"] == "attention":
                 self._mm(x, lw["qkv"], self.qkv)                                    # [B, 2048]: q | k | v
-                ctx = self.attn[lw["att"]].step(lw["att"], self.qkv, self.past, self.seq, self.tables)
+                ctx = self._attend(lw["att"], self.qkv)
                 self._mm(ctx.reshape(b, cfg.heads * cfg.head_dim), lw["out"], o)
             else:
                 self._mm(x, lw["in"], self.bcx)                                     # [B, 3 * hidden]: B | C | x
@@ -191,7 +236,7 @@ class LFM2DecodeRunner:
             block.add_rmsnorm(o, h, nxt, cfg.eps, out=x, sum_out=h)             # h += ffn; x = next norm(h)
         self._mm(x, self.head, self.logits)
         block.argmax_rows(self.logits, out=self.next_ids)
-        self.past.add_(1)
+        self._advance()
 
     def _proj(self, a: torch.Tensor, w: torch.Tensor, **tiling) -> torch.Tensor:
         """a @ w.T into a new tensor: b2_gemm, or cuBLAS with own_gemm=False."""
@@ -213,7 +258,7 @@ class LFM2DecodeRunner:
             x = rms_norm(h, lw["op_norm"], cfg.eps)
             if lw["kind"] == "attention":
                 qkv = self._proj(x, lw["qkv"])                      # [B, 2048]: q | k | v
-                ctx = self.attn[lw["att"]].step(lw["att"], qkv, self.past, self.seq, self.tables)
+                ctx = self._attend(lw["att"], qkv)
                 o = self._proj(ctx.reshape(b, cfg.heads * cfg.head_dim), lw["out"])
             else:
                 bcx = self._proj(x, lw["in"])                       # [B, 3 * hidden]: B | C | x
@@ -237,7 +282,7 @@ class LFM2DecodeRunner:
         else:
             torch.matmul(h, self.head.t(), out=self.logits)
         torch.argmax(self.logits, dim=-1, out=self.next_ids)
-        self.past.add_(1)
+        self._advance()
 
     def _run(self) -> None:
         if not self.use_graph:
@@ -266,6 +311,8 @@ class LFM2DecodeRunner:
 
     def reset(self) -> None:
         """Forget every sequence (KV lengths and conv states back to zero)."""
+        if self.block_tables is not None:
+            self.block_tables.release(torch.ones(self.max_batch, dtype=torch.bool, device=self.device))
         self.past.zero_()
         self.conv_state.zero_()
         self.position = 0
@@ -303,11 +350,19 @@ class LFM2DecodeRunner:
     def kv(self, att_index: int, seq: int, position: int):
         """(keys, values) [8, position + 1, 64] of one attention layer and sequence
         (experiments/lfm25_x8_model.py:85-92)."""
+        if self.block_tables is not None:
+            return self.cache.read_blocks(att_index, self.tables[seq], position + 1)
         return self.cache.read_dense(att_index, seq, position + 1)
 
     def check(self) -> None:
         for a in self.attn:
             a.check()
+        if self.block_tables is not None:
+            self.block_tables.check()
+            refused = int(self._refused.item())
+            if refused:
+                self._refused.zero_()
+                raise RuntimeError(f"KV pool exhausted: {refused} tokens got no block and were not cached")
         word = int(self.gemm_err.item())
         if word:
             self.gemm_err.zero_()

@@ -230,8 +230,13 @@ class PagedKVCache8(PagedKVCache):
     def read_dense(self, layer: int, seq: int, length: int) -> tuple[torch.Tensor, torch.Tensor]:
         """[8, length, 64] bf16 K and V of one sequence, the values its codes
         stand for (bf16 holds a code times its scale exactly)."""
+        return self.read_blocks(layer, self._tables[seq], length)
+
+    def read_blocks(self, layer: int, blocks, length: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """read_dense of a sequence whose blocks are not this cache's own (a
+        device block table's row)."""
         nb = blocks_for(length)
-        ids = torch.tensor(self._tables[seq][:nb], device=self.device, dtype=torch.long)
+        ids = torch.as_tensor(blocks, device=self.device).long()[:nb]
         out = []
         for pool, scale, dim_major in ((self.k, self.k_scale, False), (self.v, self.v_scale, True)):
             x = pool[layer].view(torch.uint8)[ids].view(torch.float8_e4m3fn).float() * scale[layer][ids][..., None, None]
