@@ -14,7 +14,7 @@ in the caller's `dev_err` word.
 """
 from __future__ import annotations
 
-import contextlib
+import ctypes
 
 import torch
 
@@ -26,60 +26,104 @@ from .rope import rope_table
 NORM_ROPE_STORE = _lib.B2_NORM_QK | _lib.B2_ROPE_QK | _lib.B2_STORE_KV
 
 
-def _on(device: torch.device):
-    """Launches go to the current device: make it the tensors' own."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+# The smallest calls are bound by the host.  The native binding (_b2torch, built
+# against the installed torch) checks a call's tensors and makes the library call
+# in about 2 us; where it is not built, or says None to an argument, the checks
+# below do the same: each is one comparison of what the tensor says about itself
+# (its device by index), and the slow path that words the refusal is taken only
+# when one fails.
+try:
+    from . import _b2torch
+except ImportError:
+    _b2torch = None
+_bound = None       # the library whose functions the binding holds
 
 
-def _raw_stream(device: torch.device, stream: torch.cuda.Stream | None) -> int:
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+def _native(t, stream: torch.cuda.Stream | None):
+    """The native binding and the stream for a call whose tensors are with `t`, if that is the current device."""
+    global _bound
+    if _b2torch is None or not isinstance(t, torch.Tensor):
+        return None, 0
+    index = t.get_device()
+    if index < 0 or index != torch._C._cuda_getDevice():
+        return None, 0
+    if _bound is None or _bound is not _lib._LIB:
+        lib = _lib.load()
+        _b2torch.bind(*(ctypes.cast(getattr(lib, f), ctypes.c_void_p).value for f in
+                        ("b2_kv8_decode_step", "b2_kv8_append", "b2_kv8_prefill_attn", "b2_tables_extend")))
+        _bound = lib
+    return _b2torch, torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
 
 
-def _addr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
+_I32, _F32, _BF16, _E4M3 = torch.int32, torch.float32, torch.bfloat16, torch.float8_e4m3fn
 
 
-def _is(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple) -> None:
-    """_need with the checks that pass made cheap."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or t.shape != shape or \
-            not t.is_contiguous():
-        _need(t, name, dtype, device, shape)
+def _is(t: torch.Tensor, name: str, dtype: torch.dtype, like: torch.Tensor, index: int, shape: tuple) -> int:
+    """Address of a contiguous tensor of this type and shape on like's device (index `index`)."""
+    if t.__class__ is torch.Tensor and t.dtype is dtype and t.get_device() == index and t.shape == shape and \
+            t.is_contiguous():
+        return t.data_ptr()
+    _need(t, name, dtype, like.device, shape)      # (a parameter or another subclass passes here)
+    return t.data_ptr()
 
 
-def _need_cache(k_pool, v_pool, k_scale, v_scale, device: torch.device) -> int:
+def _launch(call: str, index: int, stream: torch.cuda.Stream | None, *args) -> None:
+    """One library call on the device with this index, which is made current for it, on `stream` or the
+    device's current one."""
+    if index < 0:
+        raise ValueError(f"{call}: tensors must be on a CUDA device")
+    fn = getattr(_lib.load(), call)
+    raw = torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, raw)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, raw)
+    if rc:
+        _lib.check(rc, call)
+
+
+def _need_cache(k_pool, v_pool, k_scale, v_scale, like: torch.Tensor, index: int) -> tuple:
+    """Addresses of the pools and scales, and the number of blocks."""
     blocks = k_pool.shape[0] if isinstance(k_pool, torch.Tensor) and k_pool.dim() == 4 else 0
-    _is(k_pool, "k_pool", torch.float8_e4m3fn, device, (blocks, HKV, BLOCK, D))
-    _is(v_pool, "v_pool", torch.float8_e4m3fn, device, (blocks, HKV, D, BLOCK))
-    _is(k_scale, "k_scale", torch.float32, device, (blocks, HKV))
-    _is(v_scale, "v_scale", torch.float32, device, (blocks, HKV))
-    return blocks
+    return (_is(k_pool, "k_pool", _E4M3, like, index, (blocks, HKV, BLOCK, D)),
+            _is(v_pool, "v_pool", _E4M3, like, index, (blocks, HKV, D, BLOCK)),
+            _is(k_scale, "k_scale", _F32, like, index, (blocks, HKV)),
+            _is(v_scale, "v_scale", _F32, like, index, (blocks, HKV)), blocks)
 
 
-def _need_tables(block_tables, past_lens, chunk_lens, device: torch.device) -> tuple[int, int]:
+def _need_tables(block_tables, past_lens, chunk_lens, like: torch.Tensor, index: int) -> tuple:
+    """Batch, table width, and the addresses of tables, past and chunk lengths."""
     if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
         raise ValueError("block_tables must be [batch, max_blocks_per_seq]")
     b, width = block_tables.shape
-    _is(block_tables, "block_tables", torch.int32, device, (b, width))
-    _is(past_lens, "past_lens", torch.int32, device, (b,))
-    if chunk_lens is not None:
-        _is(chunk_lens, "chunk_lens", torch.int32, device, (b,))
-    return b, width
+    return (b, width, _is(block_tables, "block_tables", _I32, like, index, (b, width)),
+            _is(past_lens, "past_lens", _I32, like, index, (b,)),
+            None if chunk_lens is None else _is(chunk_lens, "chunk_lens", _I32, like, index, (b,)))
 
 
-def _need_qk(mode: int, gamma_q, gamma_k, cos, sin, device: torch.device) -> int:
+def _need_qk(mode: int, gamma_q, gamma_k, eps: float, cos, sin, like: torch.Tensor, index: int) -> tuple:
+    """The q/k norm and RoPE arguments of a call."""
+    gq = gk = c = s = None
+    rows = 0
     if mode & _lib.B2_NORM_QK:
-        _is(gamma_q, "gamma_q", torch.bfloat16, device, (D,))
-        _is(gamma_k, "gamma_k", torch.bfloat16, device, (D,))
-    return _need_rope(cos, sin, device) if mode & _lib.B2_ROPE_QK else 0
+        gq = _is(gamma_q, "gamma_q", _BF16, like, index, (D,))
+        gk = _is(gamma_k, "gamma_k", _BF16, like, index, (D,))
+    if mode & _lib.B2_ROPE_QK:
+        rows = _need_rope(cos, sin, like.device)
+        c, s = cos.data_ptr(), sin.data_ptr()
+    return gq, gk, eps, c, s, rows
 
 
-def _need_workspace(workspace, device: torch.device) -> int:
-    if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or workspace.device != device or \
-            not workspace.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device} (workspace_kv8)")
-    return workspace.numel()
+def _need_err(dev_err, like: torch.Tensor, index: int) -> int:
+    return _is(dev_err, "dev_err", _I32, like, index, (1,))
+
+
+def _need_workspace(workspace, like: torch.Tensor, index: int) -> tuple:
+    if not isinstance(workspace, torch.Tensor) or workspace.dtype is not torch.uint8 or \
+            workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {like.device} (workspace_kv8)")
+    return workspace.data_ptr(), workspace.numel()
 
 
 def workspace_kv8(device: torch.device | str) -> torch.Tensor:
@@ -104,34 +148,29 @@ def append_kv8(qkv: torch.Tensor, *, k_pool: torch.Tensor | None = None, v_pool:
     [rows, 16, 64] normalised and rotated query."""
     if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3) or qkv.shape[-1] < QKV_WIDTH:
         raise ValueError(f"qkv must be [rows or batch x tokens, >= {QKV_WIDTH}]")
-    dev = qkv.device
-    _need(qkv, "qkv", torch.bfloat16, dev)
-    width = qkv.shape[-1]
+    index, shape = qkv.get_device(), qkv.shape
+    width = shape[-1]
     rows = qkv.numel() // width
+    q = _is(qkv, "qkv", _BF16, qkv, index, shape)
     tokens = table_width = 0
+    slot = place = past = chunk = tables = None
     if slots is not None:
-        _is(slots, "slots", torch.int32, dev, (rows,))
+        slot = _is(slots, "slots", _I32, qkv, index, (rows,))
         if positions is not None:
-            _is(positions, "positions", torch.int32, dev, (rows,))
+            place = _is(positions, "positions", _I32, qkv, index, (rows,))
     else:
-        if qkv.dim() != 3:
+        if len(shape) != 3:
             raise ValueError("without slots, qkv must be [batch, tokens, width]")
-        b, table_width = _need_tables(block_tables, past_lens, chunk_lens, dev)
-        tokens = qkv.shape[1]
-        if b != qkv.shape[0]:
-            raise ValueError(f"block_tables must have {qkv.shape[0]} rows, got {b}")
-    blocks = _need_cache(k_pool, v_pool, k_scale, v_scale, dev) if mode & _lib.B2_STORE_KV or slots is not None else 0
-    if q_out is not None:
-        _is(q_out, "q_out", torch.bfloat16, dev, (rows, HQ, D))
-    rope_rows = _need_qk(mode, gamma_q, gamma_k, cos, sin, dev)
-    _need(dev_err, "dev_err", torch.int32, dev)
-    with _on(dev):
-        rc = _lib.load().b2_kv8_append(
-            qkv.data_ptr(), width, rows, _addr(slots), _addr(positions), _addr(past_lens), _addr(chunk_lens), tokens,
-            _addr(block_tables), table_width, _addr(gamma_q), _addr(gamma_k), eps, _addr(cos), _addr(sin), rope_rows,
-            _addr(k_pool), _addr(v_pool), _addr(k_scale), _addr(v_scale), blocks, _addr(q_out), mode,
-            dev_err.data_ptr(), _raw_stream(dev, stream))
-    _lib.check(rc, "b2_kv8_append")
+        b, table_width, tables, past, chunk = _need_tables(block_tables, past_lens, chunk_lens, qkv, index)
+        tokens = shape[1]
+        if b != shape[0]:
+            raise ValueError(f"block_tables must have {shape[0]} rows, got {b}")
+    cache = _need_cache(k_pool, v_pool, k_scale, v_scale, qkv, index) \
+        if mode & _lib.B2_STORE_KV or slots is not None else (None, None, None, None, 0)
+    q_to = None if q_out is None else _is(q_out, "q_out", _BF16, qkv, index, (rows, HQ, D))
+    _launch("b2_kv8_append", index, stream, q, width, rows, slot, place, past, chunk, tokens, tables, table_width,
+            *_need_qk(mode, gamma_q, gamma_k, eps, cos, sin, qkv, index), *cache, q_to, mode,
+            _need_err(dev_err, qkv, index))
 
 
 def decode_step_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -145,28 +184,29 @@ def decode_step_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch
     positions past_lens[b] + t, chunk_lens[b] (0 to T; None: T) of them there.
     Appends their k/v and writes the contexts into out [B, T, 16, 64]; rows
     past a sequence's chunk stay as they were.  `mode` as decode_step's."""
+    native, raw = _native(qkv, stream)
+    if native is not None:
+        rc = native.step(qkv, past_lens, k_pool, v_pool, k_scale, v_scale, block_tables, out, workspace, dev_err,
+                         chunk_lens, gamma_q, gamma_k, cos, sin, mode, eps, scale, raw)
+        if rc == 0:
+            return
+        if rc is not None:
+            _lib.check(rc, "b2_kv8_decode_step")
     if not isinstance(qkv, torch.Tensor) or qkv.dim() != 3 or qkv.shape[2] < QKV_WIDTH:
         raise ValueError(f"qkv must be [batch, tokens, >= {QKV_WIDTH}]")
-    dev = qkv.device
     b, t, width = qkv.shape
     if not 1 <= t <= MAX_STEP_TOKENS:
         raise ValueError(f"tokens must be in [1, {MAX_STEP_TOKENS}], got {t}")
-    _is(qkv, "qkv", torch.bfloat16, dev, (b, t, width))
-    tb, table_width = _need_tables(block_tables, past_lens, chunk_lens, dev)
+    index = qkv.get_device()
+    q = _is(qkv, "qkv", _BF16, qkv, index, (b, t, width))
+    tb, table_width, tables, past, chunk = _need_tables(block_tables, past_lens, chunk_lens, qkv, index)
     if tb != b:
         raise ValueError(f"block_tables must have {b} rows, got {tb}")
-    blocks = _need_cache(k_pool, v_pool, k_scale, v_scale, dev)
-    _is(out, "out", torch.bfloat16, dev, (b, t, HQ, D))
-    _need(dev_err, "dev_err", torch.int32, dev)
-    rope_rows = _need_qk(mode, gamma_q, gamma_k, cos, sin, dev)
-    nbytes = _need_workspace(workspace, dev)
-    with _on(dev):
-        rc = _lib.load().b2_kv8_decode_step(
-            qkv.data_ptr(), width, t, _addr(chunk_lens), _addr(gamma_q), _addr(gamma_k), eps, _addr(cos), _addr(sin),
-            rope_rows, past_lens.data_ptr(), block_tables.data_ptr(), table_width, k_pool.data_ptr(),
-            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, b, scale, mode, out.data_ptr(),
-            workspace.data_ptr(), nbytes, dev_err.data_ptr(), _raw_stream(dev, stream))
-    _lib.check(rc, "b2_kv8_decode_step")
+    _launch("b2_kv8_decode_step", index, stream, q, width, t, chunk,
+            *_need_qk(mode, gamma_q, gamma_k, eps, cos, sin, qkv, index), past, tables, table_width,
+            *_need_cache(k_pool, v_pool, k_scale, v_scale, qkv, index), b, scale, mode,
+            _is(out, "out", _BF16, qkv, index, (b, t, HQ, D)), *_need_workspace(workspace, qkv, index),
+            _need_err(dev_err, qkv, index))
 
 
 def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -189,12 +229,25 @@ def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Ten
 
     Returns the contexts [rows, 16, 64] ([B, T, 16, 64] for padded qkv) in
     `out` when given; rows of no token stay as they were (zero without `out`)."""
+    native, raw = _native(qkv, stream) if out is not None else (None, 0)
+    if native is not None and qkv.dim() >= 2 and qkv.shape[-1] >= QKV_WIDTH:
+        q_buf = None
+        if mode & (_lib.B2_NORM_QK | _lib.B2_ROPE_QK):
+            q_buf = torch.empty(qkv.numel() // qkv.shape[-1], HQ, D, dtype=_BF16, device=qkv.device)
+        rc = native.prefill(qkv, past_lens, k_pool, v_pool, k_scale, v_scale, block_tables, out, workspace, dev_err,
+                            chunk_lens, gamma_q, gamma_k, cos, sin, mode, eps, scale, raw, row_start, max_tokens, slots,
+                            positions, q_buf)
+        if rc == 0:
+            return out
+        if rc is not None:
+            _lib.check(rc, "b2_kv8_append / b2_kv8_prefill_attn")
     if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3) or qkv.shape[-1] < QKV_WIDTH:
         raise ValueError(f"qkv must be [rows, >= {QKV_WIDTH}] or [batch, tokens, >= {QKV_WIDTH}]")
-    dev = qkv.device
+    index = qkv.get_device()
     width = qkv.shape[-1]
     rows = qkv.numel() // width
-    b, table_width = _need_tables(block_tables, past_lens, chunk_lens, dev)
+    b, table_width, tables, past, chunk = _need_tables(block_tables, past_lens, chunk_lens, qkv, index)
+    start = None
     if qkv.dim() == 3:
         tokens = qkv.shape[1]
         if qkv.shape[0] != b or row_start is not None:
@@ -203,30 +256,27 @@ def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Ten
     else:
         if row_start is None or max_tokens is None or slots is None:
             raise ValueError("packed qkv needs row_start, max_tokens and slots")
-        _is(row_start, "row_start", torch.int32, dev, (b,))
+        start = _is(row_start, "row_start", _I32, qkv, index, (b,))
         tokens = int(max_tokens)
         shape = (rows, HQ, D)
     if out is None:
-        out = torch.zeros(shape, dtype=torch.bfloat16, device=dev)
-    _is(out, "out", torch.bfloat16, dev, shape)
-    blocks = _need_cache(k_pool, v_pool, k_scale, v_scale, dev)
-    nbytes = _need_workspace(workspace, dev)
+        out = torch.zeros(shape, dtype=_BF16, device=qkv.device)
+    to = _is(out, "out", _BF16, qkv, index, shape)
+    cache = _need_cache(k_pool, v_pool, k_scale, v_scale, qkv, index)
+    work = _need_workspace(workspace, qkv, index)
+    err = _need_err(dev_err, qkv, index)
+    q = _is(qkv, "qkv", _BF16, qkv, index, qkv.shape)
+    slot = None if slots is None else _is(slots, "slots", _I32, qkv, index, (rows,))
+    place = None if positions is None else _is(positions, "positions", _I32, qkv, index, (rows,))
+    qk = _need_qk(mode, gamma_q, gamma_k, eps, cos, sin, qkv, index)
     turned = mode & (_lib.B2_NORM_QK | _lib.B2_ROPE_QK)
-    q = torch.empty(rows, HQ, D, dtype=torch.bfloat16, device=dev) if turned else None
+    q_buf = torch.empty(rows, HQ, D, dtype=_BF16, device=qkv.device) if turned else None
     if mode:
-        append_kv8(qkv, k_pool=k_pool, v_pool=v_pool, k_scale=k_scale, v_scale=v_scale, dev_err=dev_err, slots=slots,
-                   positions=positions, past_lens=past_lens, block_tables=block_tables, chunk_lens=chunk_lens,
-                   q_out=q, gamma_q=gamma_q, gamma_k=gamma_k, cos=cos, sin=sin, mode=mode, eps=eps, stream=stream)
-    else:
-        _need(qkv, "qkv", torch.bfloat16, dev)
-        _need(dev_err, "dev_err", torch.int32, dev)
-    with _on(dev):
-        rc = _lib.load().b2_kv8_prefill_attn(
-            qkv.data_ptr() if q is None else q.data_ptr(), width if q is None else HQ * D, rows, _addr(row_start),
-            past_lens.data_ptr(), _addr(chunk_lens), tokens, block_tables.data_ptr(), table_width, k_pool.data_ptr(),
-            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), blocks, b, scale, out.data_ptr(),
-            workspace.data_ptr(), nbytes, dev_err.data_ptr(), _raw_stream(dev, stream))
-    _lib.check(rc, "b2_kv8_prefill_attn")
+        _launch("b2_kv8_append", index, stream, q, width, rows, slot, place, past, chunk, tokens, tables, table_width,
+                *qk, *cache, None if q_buf is None else q_buf.data_ptr(), mode, err)
+    _launch("b2_kv8_prefill_attn", index, stream, q if q_buf is None else q_buf.data_ptr(),
+            width if q_buf is None else HQ * D, rows, start, past, chunk, tokens, tables, table_width, *cache, b, scale,
+            to, *work, err)
     return out
 
 

@@ -18,8 +18,14 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention_kv8 import _addr, _is, _on, _raw_stream
+from .attention_kv8 import _I32, _is, _launch, _native
 from .paged_cache import blocks_for
+
+
+def _table_shape(block_tables) -> torch.Size:
+    if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
+        raise ValueError("block_tables must be [batch, max_blocks_per_seq]")
+    return block_tables.shape
 
 
 def extend_tables(block_tables: torch.Tensor, held: torch.Tensor, free_list: torch.Tensor, free_count: torch.Tensor,
@@ -34,34 +40,31 @@ def extend_tables(block_tables: torch.Tensor, held: torch.Tensor, free_list: tor
     first row of each, slots / positions [rows] the slot (block * 64 + row; -1
     for no token) and position of each row.  tokens_per_seq: 0 for packed rows,
     T for rows b * T + t."""
-    dev = block_tables.device
-    if block_tables.dim() != 2 or not isinstance(slots, torch.Tensor):
-        raise ValueError("block_tables must be [batch, max_blocks_per_seq], slots a tensor")
-    b, width = block_tables.shape
-    rows = slots.numel()
-    held_out = held if held_out is None else held_out
-    free_count_out = free_count if free_count_out is None else free_count_out
-    i32 = torch.int32
-    _is(block_tables, "block_tables", i32, dev, (b, width))
-    _is(held, "held", i32, dev, (b,))
-    _is(free_list, "free_list", i32, dev, (free_list.numel(),))
-    _is(free_count, "free_count", i32, dev, (1,))
-    _is(past_lens, "past_lens", i32, dev, (b,))
-    _is(new_lens, "new_lens", i32, dev, (b,))
-    _is(held_out, "held_out", i32, dev, (b,))
-    _is(free_count_out, "free_count_out", i32, dev, (1,))
-    _is(granted, "granted", i32, dev, (b,))
-    _is(row_start, "row_start", i32, dev, (b,))
-    _is(slots, "slots", i32, dev, (rows,))
-    _is(positions, "positions", i32, dev, (rows,))
-    _is(dev_err, "dev_err", i32, dev, (1,))
-    with _on(dev):
-        rc = _lib.load().b2_tables_extend(
-            block_tables.data_ptr(), width, held.data_ptr(), free_list.data_ptr(), free_list.numel(),
-            free_count.data_ptr(), past_lens.data_ptr(), new_lens.data_ptr(), b, held_out.data_ptr(),
-            free_count_out.data_ptr(), granted.data_ptr(), row_start.data_ptr(), slots.data_ptr(),
-            positions.data_ptr(), rows, tokens_per_seq, dev_err.data_ptr(), _raw_stream(dev, stream))
-    _lib.check(rc, "b2_tables_extend")
+    native, raw = _native(block_tables, stream)
+    if native is not None:
+        rc = native.extend(block_tables, held, free_list, free_count, past_lens, new_lens, held_out, free_count_out,
+                           granted, row_start, slots, positions, tokens_per_seq, dev_err, raw)
+        if rc == 0:
+            return
+        if rc is not None:
+            _lib.check(rc, "b2_tables_extend")
+    b, width = _table_shape(block_tables)
+    rows, blocks = slots.numel(), free_list.numel()
+    index, per_b = block_tables.get_device(), (b,)
+    held_at = _is(held, "held", _I32, block_tables, index, per_b)
+    count_at = _is(free_count, "free_count", _I32, block_tables, index, (1,))
+    _launch("b2_tables_extend", index, stream,
+            _is(block_tables, "block_tables", _I32, block_tables, index, (b, width)), width, held_at,
+            _is(free_list, "free_list", _I32, block_tables, index, (blocks,)), blocks, count_at,
+            _is(past_lens, "past_lens", _I32, block_tables, index, per_b),
+            _is(new_lens, "new_lens", _I32, block_tables, index, per_b), b,
+            held_at if held_out is None else _is(held_out, "held_out", _I32, block_tables, index, per_b),
+            count_at if free_count_out is None else _is(free_count_out, "free_count_out", _I32, block_tables, index, (1,)),
+            _is(granted, "granted", _I32, block_tables, index, per_b),
+            _is(row_start, "row_start", _I32, block_tables, index, per_b),
+            _is(slots, "slots", _I32, block_tables, index, (rows,)),
+            _is(positions, "positions", _I32, block_tables, index, (rows,)), rows, tokens_per_seq,
+            _is(dev_err, "dev_err", _I32, block_tables, index, (1,)))
 
 
 def slot_map(block_tables: torch.Tensor, past_lens: torch.Tensor, new_lens: torch.Tensor, *, num_blocks: int,
@@ -71,47 +74,31 @@ def slot_map(block_tables: torch.Tensor, past_lens: torch.Tensor, new_lens: torc
     """Slots and positions of new_lens[b] tokens behind past_lens[b] from tables
     whose blocks are there (b2_slot_map): rows from row_start[b] on (ascending,
     not overlapping), or rows b * tokens_per_seq + t."""
-    dev = block_tables.device
-    if block_tables.dim() != 2 or not isinstance(slots, torch.Tensor):
-        raise ValueError("block_tables must be [batch, max_blocks_per_seq], slots a tensor")
-    b, width = block_tables.shape
-    rows = slots.numel()
-    i32 = torch.int32
-    _is(block_tables, "block_tables", i32, dev, (b, width))
-    _is(past_lens, "past_lens", i32, dev, (b,))
-    _is(new_lens, "new_lens", i32, dev, (b,))
-    if row_start is not None:
-        _is(row_start, "row_start", i32, dev, (b,))
-    _is(slots, "slots", i32, dev, (rows,))
-    _is(positions, "positions", i32, dev, (rows,))
-    _is(dev_err, "dev_err", i32, dev, (1,))
-    with _on(dev):
-        rc = _lib.load().b2_slot_map(
-            block_tables.data_ptr(), width, num_blocks, past_lens.data_ptr(), new_lens.data_ptr(), _addr(row_start),
-            b, slots.data_ptr(), positions.data_ptr(), rows, tokens_per_seq, dev_err.data_ptr(),
-            _raw_stream(dev, stream))
-    _lib.check(rc, "b2_slot_map")
+    b, width = _table_shape(block_tables)
+    rows, index, per_b = slots.numel(), block_tables.get_device(), (b,)
+    _launch("b2_slot_map", index, stream,
+            _is(block_tables, "block_tables", _I32, block_tables, index, (b, width)), width, num_blocks,
+            _is(past_lens, "past_lens", _I32, block_tables, index, per_b),
+            _is(new_lens, "new_lens", _I32, block_tables, index, per_b),
+            None if row_start is None else _is(row_start, "row_start", _I32, block_tables, index, per_b), b,
+            _is(slots, "slots", _I32, block_tables, index, (rows,)),
+            _is(positions, "positions", _I32, block_tables, index, (rows,)), rows, tokens_per_seq,
+            _is(dev_err, "dev_err", _I32, block_tables, index, (1,)))
 
 
 def release_tables(block_tables: torch.Tensor, held: torch.Tensor, free_list: torch.Tensor, free_count: torch.Tensor,
                    finished: torch.Tensor, *, dev_err: torch.Tensor, stream: torch.cuda.Stream | None = None) -> None:
     """Blocks of the requests with finished[b] (bool [B]) back to the free list
     (b2_tables_release); their rows become -1 and held[b] 0."""
-    dev = block_tables.device
-    if block_tables.dim() != 2:
-        raise ValueError("block_tables must be [batch, max_blocks_per_seq]")
-    b, width = block_tables.shape
-    _is(block_tables, "block_tables", torch.int32, dev, (b, width))
-    _is(held, "held", torch.int32, dev, (b,))
-    _is(free_list, "free_list", torch.int32, dev, (free_list.numel(),))
-    _is(free_count, "free_count", torch.int32, dev, (1,))
-    _is(finished, "finished", torch.bool, dev, (b,))
-    _is(dev_err, "dev_err", torch.int32, dev, (1,))
-    with _on(dev):
-        rc = _lib.load().b2_tables_release(
-            block_tables.data_ptr(), width, held.data_ptr(), free_list.data_ptr(), free_list.numel(),
-            free_count.data_ptr(), finished.data_ptr(), b, dev_err.data_ptr(), _raw_stream(dev, stream))
-    _lib.check(rc, "b2_tables_release")
+    b, width = _table_shape(block_tables)
+    index, blocks = block_tables.get_device(), free_list.numel()
+    _launch("b2_tables_release", index, stream,
+            _is(block_tables, "block_tables", _I32, block_tables, index, (b, width)), width,
+            _is(held, "held", _I32, block_tables, index, (b,)),
+            _is(free_list, "free_list", _I32, block_tables, index, (blocks,)), blocks,
+            _is(free_count, "free_count", _I32, block_tables, index, (1,)),
+            _is(finished, "finished", torch.bool, block_tables, index, (b,)), b,
+            _is(dev_err, "dev_err", _I32, block_tables, index, (1,)))
 
 
 @dataclass

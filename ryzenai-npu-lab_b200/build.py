@@ -1,4 +1,5 @@
-"""Build libb2attn.so in-tree with nvcc for sm_100a.
+"""Build libb2attn.so in-tree with nvcc for sm_100a, and the native binding
+_b2torch.so of its smallest calls with g++.
 
 The shared library is the product's compute path: it holds every CUDA kernel
 and the C ABI declared in the headers of include/.  It is built next to this file so that it travels with the source tree to the GPU host.
@@ -14,6 +15,8 @@ PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libb2attn.so"
+BINDING = PKG / "_b2torch.so"
+BINDING_SOURCE = CSRC / "b2_torch.cpp"
 SOURCES = [CSRC / "b2_attn.cu", CSRC / "b2_block.cu", CSRC / "b2_gemm.cu",
            CSRC / "b2_kv8.cu", CSRC / "b2_tables.cu"]
 HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h",
@@ -42,8 +45,43 @@ def needs_build(lib: pathlib.Path = LIB) -> bool:
     return any(p.stat().st_mtime > mtime for p in SOURCES + HEADERS)
 
 
+def _start_binding(force: bool):
+    """The compilation of the binding against the installed torch, started; None when up to date."""
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > BINDING_SOURCE.stat().st_mtime:
+        return None
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    tmp = BINDING.with_suffix(".so.tmp")
+    lib = pathlib.Path(torch.__file__).parent / "lib"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DNDEBUG",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in include_paths()), f"-I{sysconfig.get_paths()['include']}", str(BINDING_SOURCE),
+           f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    return tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _finish_binding(started) -> None:
+    if started is None:
+        return
+    tmp, proc = started
+    text, _ = proc.communicate()
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{text}")
+    os.replace(tmp, BINDING)
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
-    """Compile the CUDA sources into libb2attn.so (skipped when up to date)."""
+    """Compile the CUDA sources into libb2attn.so and the binding (each skipped when up to date)."""
+    binding = _start_binding(force)
+    try:
+        return _build_library(force, verbose)
+    finally:
+        _finish_binding(binding)
+
+
+def _build_library(force: bool, verbose: bool) -> pathlib.Path:
     if not force and not needs_build():
         return LIB
     tmp = LIB.with_suffix(".so.tmp")
