@@ -121,9 +121,15 @@ struct AppendArgs {
   int32_t *err;
 };
 
-constexpr int kWindow = 8;                          // rows whose runs start in one CTA
-constexpr int kSeen = 1 + kWindow + kBlock;         // the row before, the window, and a run's rows behind it
+constexpr int kMaxWindow = 64;   // rows whose runs start in one CTA: 8 or 64
 constexpr int kNoSlot = -1;
+constexpr int kAppendThreads = 512;
+
+// A run's rows of one head, K or V, per warp, and the places of the rows around.
+struct AppendShared {
+  uint16_t rows[kAppendThreads / 32][kBlock][kDim];
+  int slot[1 + kMaxWindow + kBlock], place[1 + kMaxWindow + kBlock];  // entry i: row row0 - 1 + i
+};
 
 // Slot and RoPE position of a row; kNoSlot for a row to skip.
 __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &position, int &flag) {
@@ -160,122 +166,159 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
   return blk * kBlock + static_cast<int>(pos % kBlock);
 }
 
-// One CTA per window of rows, warp = KV head.  A run is a sequence of adjacent
-// rows that go to adjacent slots of one block; the warp whose window holds
-// the run's first row quantises the whole run for its head, so a block's scale
-// is found and its codes are written by one warp alone, with no atomics.
-// 8 lanes own one 64-wide head vector, 8 values each (four rows per pass).
-__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
-  __shared__ int slot[kSeen], place[kSeen];  // entry i: row row0 - 1 + i
-  const int row0 = blockIdx.x * kWindow;
+// One CTA per window of rows, warp = (KV head, K or V).  A run is a sequence of
+// adjacent rows that go to adjacent slots of one block; the warps of the window
+// that holds its first row quantise the whole run, each for its head, so a
+// block's scale is found and its codes are written by one warp alone, with no
+// atomics.  All of a run's loads are in flight together (up to 16 per lane; 8
+// lanes own one 64-wide head vector) on their way to shared memory, from where
+// norm and RoPE, the maximum and the codes are taken.  Codes leave in 16-byte
+// pieces: a lane takes 16 dims of a K row, or 16 tokens of two V dims, for which
+// shared memory is the transpose.
+//
+// Bound by latency for the few rows of a short prompt and by the reads of qkv
+// for long ones.  kWindow 8 spreads few rows over the SMs; 64 keeps the CTAs
+// that hold no run's start from outnumbering the others in long prompts.
+template <int kWindow>
+__global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const AppendArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  AppendShared &sh = *reinterpret_cast<AppendShared *>(smem_raw);
+  const int row0 = static_cast<int>(blockIdx.x) * kWindow;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = lane & 7, grp = lane >> 3;
-  for (int i = threadIdx.x; i < kSeen; i += 256) {
-    const int r = row0 - 1 + i;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int i = threadIdx.x; i < 1 + kWindow + kBlock; i += kAppendThreads) {
+    const int64_t r = static_cast<int64_t>(row0) - 1 + i;
     int position = 0, flag = 0;
-    slot[i] = r >= 0 && r < a.rows ? row_place(a, r, position, flag) : kNoSlot;
-    place[i] = position;
+    sh.slot[i] = r >= 0 && r < a.rows ? row_place(a, static_cast<int>(r), position, flag) : kNoSlot;
+    sh.place[i] = position;
     if (i >= 1 && i <= kWindow) {
-      if (slot[i] >= 0 && (a.mode & B2_ROPE_QK) && (position < 0 || position >= a.rope_rows)) flag |= B2_DEV_BAD_POSITION;
+      if (sh.slot[i] >= 0 && (a.mode & B2_ROPE_QK) && (position < 0 || position >= a.rope_rows))
+        flag |= B2_DEV_BAD_POSITION;
       if (flag) atomicOr(a.err, flag);
     }
   }
   __syncthreads();
-
-  // head vector `vec` of row r as this lane's 8 values, normalised and rotated
-  auto load = [&](int r, int i, int vec, bool norm, const uint16_t *gamma, bool rope, float x[8]) {
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (r >= 0) w = *reinterpret_cast<const uint4 *>(a.qkv + static_cast<int64_t>(r) * a.row_stride + vec * kDim + j * 8);
-    unpack8(w, x);
-    const int pos = place[i];
-    const bool turn = rope && pos >= 0 && pos < a.rope_rows;
-    if (norm || rope)
-      norm_rope8(x, j, norm, turn, gamma, a.eps, turn ? a.cos + static_cast<int64_t>(pos) * kDim : nullptr,
-                 turn ? a.sin + static_cast<int64_t>(pos) * kDim : nullptr);
-  };
   const bool norm = (a.mode & B2_NORM_QK) != 0, rope = (a.mode & B2_ROPE_QK) != 0;
+  // norm and RoPE of four head vectors (one per 8 lanes) of the rows at entries i
+  auto turn = [&](float x[8], int i, const uint16_t *gamma) {
+    const int pos = sh.place[i];
+    const bool on = rope && pos >= 0 && pos < a.rope_rows;
+    norm_rope8(x, j, norm, on, gamma, a.eps, on ? a.cos + static_cast<int64_t>(pos) * kDim : nullptr,
+               on ? a.sin + static_cast<int64_t>(pos) * kDim : nullptr);
+  };
 
   if (a.q_out) {
-    // warp w: the 16 query heads of row row0 + w
-    const int i = 1 + warp, r = row0 + warp;
-    if (r < a.rows && slot[i] >= 0) {
-      for (int p = 0; p < kHq / 4; ++p) {
-        const int vec = 4 * p + grp;
-        float x[8];
-        load(r, i, vec, norm, a.gamma_q, rope, x);
-        *reinterpret_cast<uint4 *>(a.q_out + (static_cast<int64_t>(r) * kHq + vec) * kDim + j * 8) = pack8(x);
-      }
+    // four query heads of a row per pass, the passes of the window's rows over the warps
+    for (int p = warp; p < kWindow * (kHq / 4); p += kAppendThreads / 32) {
+      const int i = 1 + p / (kHq / 4), vec = 4 * (p % (kHq / 4)) + grp;
+      if (sh.slot[i] < 0) continue;
+      const int64_t r = row0 - 1 + i;
+      float x[8];
+      unpack8(__ldg(reinterpret_cast<const uint4 *>(a.qkv + r * a.row_stride + vec * kDim + j * 8)), x);
+      if (norm || rope) turn(x, i, a.gamma_q);
+      *reinterpret_cast<uint4 *>(a.q_out + (r * kHq + vec) * kDim + j * 8) = pack8(x);
     }
   }
   if (!(a.mode & B2_STORE_KV)) return;
 
-  const int h = warp;
+  const int h = warp >> 1;
+  const bool is_v = warp & 1;
+  uint16_t(*rows)[kDim] = sh.rows[warp];
   for (int i0 = 1; i0 <= kWindow; ++i0) {
-    const int s0 = slot[i0];
+    const int s0 = sh.slot[i0];
     if (s0 < 0) continue;
-    const int blk = s0 / kBlock, r0 = s0 % kBlock;
-    const int prev = slot[i0 - 1];
+    const int blk = s0 / kBlock, r0 = s0 % kBlock, prev = sh.slot[i0 - 1];
     if (prev >= 0 && prev + 1 == s0 && r0 != 0) continue;  // inside a run
     int n = 1;
-    while (r0 + n < kBlock && slot[i0 + n] == s0 + n) ++n;
-    const int row = row0 - 1 + i0;
-    const int64_t tile = (static_cast<int64_t>(blk) * kHkv + h) * kTile;
-    const int64_t si = static_cast<int64_t>(blk) * kHkv + h;
-    for (int which = 0; which < 2; ++which) {
-      const bool is_v = which == 1;
-      const int vec = kHq + (is_v ? kHkv : 0) + h;
-      float amax = 0.f;
-      for (int i = 0; i < n; i += 4) {
-        const bool live = i + grp < n;
-        float x[8];
-        load(live ? row + i + grp : -1, live ? i0 + i + grp : 0, vec, norm && !is_v, a.gamma_k, rope && !is_v, x);
-        if (live) {
+    while (r0 + n < kBlock && sh.slot[i0 + n] == s0 + n) ++n;
+    const uint16_t *src = a.qkv + (static_cast<int64_t>(row0) - 1 + i0 + grp) * a.row_stride +
+                          (kHq + (is_v ? kHkv : 0) + h) * kDim + j * 8;
+    uint4 w[kBlock / 4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) amax = fmaxf(amax, limited_abs(x[e]));
-        }
+    for (int i = 0; i < kBlock / 4; ++i)
+      if (4 * i + grp < n) w[i] = __ldg(reinterpret_cast<const uint4 *>(src + 4 * i * a.row_stride));
+    float amax = 0.f;
+    if (is_v || !(norm || rope)) {
+#pragma unroll
+      for (int i = 0; i < kBlock / 4; ++i) {
+        if (4 * i + grp >= n) continue;
+        float x[8];
+        unpack8(w[i], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, limited_abs(x[e]));
+        *reinterpret_cast<uint4 *>(&rows[4 * i + grp][8 * j]) = w[i];
       }
-      float *sp = (is_v ? a.v_scale : a.k_scale) + si;
-      uint8_t *codes = (is_v ? a.v_pool : a.k_pool) + tile;
-      const float old = r0 > 0 ? *sp : 0.f;
-      const float s = fmaxf(scale_for(warp_max(amax)), old);
-      if (r0 > 0 && s > old) {
-        // the rows in front of the run move to the larger scale: K rows are
-        // whole 16-byte pieces, V's are the first r0 bytes of every dim
-        const float ratio = old / s;
-        if (!is_v) {
-          for (int c = lane; c < r0 * 4; c += 32) {
-            uint4 *p = reinterpret_cast<uint4 *>(codes) + c;
-            *p = rescale16(*p, ratio, 16);
-          }
-        } else {
-          const int per = (r0 + 15) / 16;
-          for (int c = lane; c < kDim * per; c += 32) {
-            const int d = c / per, q = c - d * per;
-            uint4 *p = reinterpret_cast<uint4 *>(codes + d * kBlock) + q;
-            *p = rescale16(*p, ratio, r0 - 16 * q);
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) *sp = s;
-      const float inv = 1.0f / s;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBlock / 4; ++i)
+        if (4 * i + grp < n) *reinterpret_cast<uint4 *>(&rows[4 * i + grp][8 * j]) = w[i];
       for (int i = 0; i < n; i += 4) {
         const bool live = i + grp < n;
         float x[8];
-        load(live ? row + i + grp : -1, live ? i0 + i + grp : 0, vec, norm && !is_v, a.gamma_k, rope && !is_v, x);
+        unpack8(live ? *reinterpret_cast<const uint4 *>(&rows[i + grp][8 * j]) : make_uint4(0u, 0u, 0u, 0u), x);
+        turn(x, live ? i0 + i + grp : 0, a.gamma_k);
         if (!live) continue;
-        uint32_t c[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = e4m3x2(limited(x[2 * e]) * inv, limited(x[2 * e + 1]) * inv);
-        const int at = r0 + i + grp;
-        if (!is_v) {
-          *reinterpret_cast<uint2 *>(codes + at * kDim + j * 8) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) codes[(8 * j + e) * kBlock + at] = static_cast<uint8_t>(c[e >> 1] >> (8 * (e & 1)));
-        }
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, limited_abs(x[e]));
+        *reinterpret_cast<uint4 *>(&rows[i + grp][8 * j]) = pack8(x);
       }
     }
+    const int64_t id = static_cast<int64_t>(blk) * kHkv + h;
+    float *sp = (is_v ? a.v_scale : a.k_scale) + id;
+    uint8_t *codes = (is_v ? a.v_pool : a.k_pool) + id * kTile;
+    const float old = r0 > 0 ? *sp : 0.f;
+    const float s = fmaxf(scale_for(warp_max(amax)), old), inv = 1.0f / s;
+    const bool raise = r0 > 0 && s > old;  // the rows in front of the run move to the larger scale
+    const float ratio = raise ? old / s : 1.f;
+    __syncwarp();
+    if (lane == 0) *sp = s;
+    auto code = [&](uint32_t two) {  // two bf16 as two codes
+      return e4m3x2(limited(__uint_as_float(two << 16)) * inv, limited(__uint_as_float(two & 0xffff0000u)) * inv);
+    };
+    if (!is_v) {
+      // 4 lanes per row, 16 dims each
+      if (raise)
+        for (int c = lane; c < r0 * 4; c += 32) {
+          uint4 *p = reinterpret_cast<uint4 *>(codes) + c;
+          *p = rescale16(*p, ratio, 16);
+        }
+      for (int c = lane; c < n * 4; c += 32) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(&rows[c >> 2][16 * (c & 3)]);
+        const uint4 x = p[0], y = p[1];
+        reinterpret_cast<uint4 *>(codes)[r0 * 4 + c] =
+            make_uint4(code(x.x) | (code(x.y) << 16), code(x.z) | (code(x.w) << 16), code(y.x) | (code(y.y) << 16),
+                       code(y.z) | (code(y.w) << 16));
+      }
+    } else {
+      // dims 2 lane, 2 lane + 1; pieces of 16 tokens that hold rows of the run (or rows that move)
+      const int first = raise ? 0 : r0 / 16, last = (r0 + n - 1) / 16;
+      for (int q = first; q <= last; ++q) {
+        uint4 *p0 = reinterpret_cast<uint4 *>(codes + 2 * lane * kBlock) + q, *p1 = p0 + kBlock / 16;
+        const int lo = r0 - 16 * q, hi = r0 + n - 16 * q;  // rows of the run in this piece: [lo, hi)
+        uint32_t u[4] = {0u, 0u, 0u, 0u}, v[4] = {0u, 0u, 0u, 0u};
+        if (lo > 0 || hi < 16) {
+          uint4 x = *p0, y = *p1;
+          if (raise && lo > 0) {
+            x = rescale16(x, ratio, lo);
+            y = rescale16(y, ratio, lo);
+          }
+          u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
+          v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (i < lo || i >= hi) continue;
+          const uint32_t c = code(*reinterpret_cast<const uint32_t *>(&rows[i - lo][2 * lane]));
+          const uint32_t keep = ~(0xffu << (8 * (i & 3)));
+          u[i >> 2] = (u[i >> 2] & keep) | ((c & 0xffu) << (8 * (i & 3)));
+          v[i >> 2] = (v[i >> 2] & keep) | ((c >> 8) << (8 * (i & 3)));
+        }
+        *p0 = make_uint4(u[0], u[1], u[2], u[3]);
+        *p1 = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    __syncwarp();  // the rows may be overwritten by the next run's
   }
 }
 
@@ -331,7 +374,16 @@ constexpr int kMaxCtas = 256;
 constexpr uint64_t kDrainNs = 2000000000ull;
 constexpr float kSlack = 8.0f;          // log2 units that a score may exceed m by
 constexpr float kMaxGain = 128.0f;      // g without a look at the tile's maximum
+constexpr float kMaxGainLog2 = 7.0f;
+constexpr float kMinGainLog2 = 60.0f;   // below 2^-60 the products' sum may underflow
 constexpr float kUnset = -1.0e30f;
+
+// log2 of a scale; exact for powers of two
+__device__ __forceinline__ float log2_scale(float s) {
+  const uint32_t u = __float_as_uint(s);
+  const float e = static_cast<float>(static_cast<int>(u >> 23) - 127);
+  return (u & 0x007fffffu) == 0 ? e : e + __log2f(__uint_as_float((u & 0x007fffffu) | 0x3f800000u));
+}
 
 template <int kT>
 struct __align__(128) StepShared {
@@ -1148,6 +1200,7 @@ constexpr int kPfThreads = 7 * 32;
 constexpr int kPfTmemCols = 256;             // S at columns 0 and 64, O at 128, P at 192 and 224
 constexpr int kPfOperand = kBlock * kDim * 2;
 constexpr int kPfMaxSplit = 32;
+constexpr int kPfSortMax = 128;              // sequences that are started longest first
 constexpr int kPfMaxParts = 320;             // CTAs of a split launch
 constexpr uint32_t kPfIdesc = (1u << 4) | (8u << 17) | (8u << 24);  // f32 <- f16, M 128, N 64, both K-major
 
@@ -1216,12 +1269,30 @@ __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0
 
 __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const PrefillArgs a) {
   const int h = blockIdx.y;
-  const int b = static_cast<int>(blockIdx.z) / a.nsplit, split = static_cast<int>(blockIdx.z) - b * a.nsplit;
+  const int rank = static_cast<int>(blockIdx.z) / a.nsplit, split = static_cast<int>(blockIdx.z) - rank * a.nsplit;
   // the last tiles see the most keys: they start first
   const int tile = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x), t0 = tile * kBlock;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // .. and the longest sequences: CTAs start in the order of blockIdx, so the
+  // launch does not end on one that came late
+  int b = rank;
+  const int batch = static_cast<int>(gridDim.z) / a.nsplit;
+  if (batch > 1 && batch <= kPfSortMax) {
+    __shared__ int keys[kPfSortMax];
+    __shared__ int chosen;
+    for (int i = tid; i < batch; i += kPfThreads) keys[i] = a.past_lens[i] + (a.chunk_lens ? a.chunk_lens[i] : a.tokens);
+    __syncthreads();
+    for (int i = tid; i < batch; i += kPfThreads) {
+      const int mine = keys[i];
+      int before = 0;
+      for (int q = 0; q < batch; ++q) before += keys[q] > mine || (keys[q] == mine && q < i);
+      if (before == rank) chosen = i;
+    }
+    __syncthreads();
+    b = chosen;
+  }
   PrefillTile pt;
   if (!prefill_tile(a, b, t0, tid == 0, pt) || split >= pt.parts) return;
   const int past = pt.past, rows_t = pt.rows, last_key = past + t0 + rows_t - 1;
@@ -1472,23 +1543,20 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       for (int e = 0; e < 8; ++e) bm8[e] = sc[e];
 #pragma unroll
       for (int c = 8; c < 64; ++c) bm8[c & 7] = fmaxf(bm8[c & 7], sc[c]);
-      const float w = factor * ks;
+      const float w = fmaxf(factor * ks, 1.2e-38f);  // not 0, which would make NaN of a masked score
       const float top = fmaxf(fmaxf(fmaxf(bm8[0], bm8[1]), fmaxf(bm8[2], bm8[3])),
                               fmaxf(fmaxf(bm8[4], bm8[5]), fmaxf(bm8[6], bm8[7]))) * w;
       if (top > m + kSlack) {
         l *= ex2(m - top);
         m = top;
       }
-      const uint32_t vbits = __float_as_uint(vs);
-      const float vmant = __uint_as_float((vbits & 0x007fffffu) | 0x3f800000u);
-      const float vexp = static_cast<float>(static_cast<int>(vbits >> 23) - 127);
-      float gain = vmant * ex2(m - mo + vexp), again = 1.f;
-      if (gain > kMaxGain) {
+      const float lv = log2_scale(vs);
+      float again = 1.f;
+      if (m - mo + lv > kMaxGainLog2) {
         // the largest product so far at 1
-        const float n = fmaxf(mo, top + vexp + __log2f(vmant));
+        const float n = fmaxf(mo, top + lv);
         again = ex2(mo - n);
         mo = n;
-        gain = vmant * ex2(m - mo + vexp);
       }
       if (__any_sync(0xffffffffu, again != 1.f && j > 0)) {
         if (!warp_wait(smem_u32(&tail->pvbar), (j - 1) & 1)) {
@@ -1508,6 +1576,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
         }
         tmem_wait_st();
       }
+      const float off = lv - mo;  // p * g = 2^(score - m) * 2^(m - mo) * scale, in one exponent
       float ps[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) ps[e] = 0.f;
@@ -1515,14 +1584,28 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
         float x0, x1;
-        ffma2(x0, x1, sc[c], sc[c + 1], w, w, -m, -m);
+        ffma2(x0, x1, sc[c], sc[c + 1], w, w, off, off);
         x0 = ex2(x0);
         x1 = ex2(x1);
         const int e = c & 7;
         fadd2(ps[e], ps[e + 1], ps[e], ps[e + 1], x0, x1);
-        pk[c >> 1] = pack_f16x2(x0 * gain, x1 * gain);
+        pk[c >> 1] = pack_f16x2(x0, x1);
       }
-      l += ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+      float sum = ((ps[0] + ps[1]) + (ps[2] + ps[3])) + ((ps[4] + ps[5]) + (ps[6] + ps[7]));
+      const float low = mo - lv - m;  // -log2 of the gain
+      if (__any_sync(0xffffffffu, low > kMinGainLog2)) {
+        // a scale so far below the others' that its products underflow: the sum on its own
+        if (low > kMinGainLog2) {
+          sum = 0.f;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) sum += ex2(fmaf(sc[c], w, -m));
+          l += sum;
+        } else {
+          l = fmaf(sum, ex2(low), l);
+        }
+      } else {
+        l = fmaf(sum, ex2(low), l);
+      }
       // into buffer j % 2 once the product that read it is done
       if (j >= 2 && !warp_wait(smem_u32(&tail->pfree[j & 1]), ((j >> 1) - 1) & 1)) {
         ok = false;
@@ -1699,9 +1782,19 @@ int check_tables(const void *tables, int32_t max_blocks, const void *past_lens) 
   return B2_OK;
 }
 
+template <int kWindow>
 int launch_append(const AppendArgs &a, cudaStream_t st) {
+  static std::atomic<bool> done[128];  // the attribute is per device
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 128) return fail(B2_ERR_CUDA, "no current device");
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kv8_append_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(sizeof(AppendShared))) != cudaSuccess)
+      return fail(B2_ERR_CUDA, "cannot set the append kernel's shared memory size");
+    done[dev] = true;
+  }
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kWindow - 1) / kWindow);
-  kv8_append_kernel<<<grid, 256, 0, st>>>(a);
+  kv8_append_kernel<kWindow><<<grid, kAppendThreads, sizeof(AppendShared), st>>>(a);
   return launched(cudaSuccess, "kv8_append_kernel");
 }
 
@@ -1740,7 +1833,8 @@ extern "C" int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t ro
   AppendArgs a{qkv, row_stride, rows, slots, positions, past_lens, chunk_lens, tokens, block_tables,
                max_blocks_per_seq, gamma_q, gamma_k, eps, rope_cos, rope_sin, rope_rows, k_pool, v_pool,
                k_scale, v_scale, num_blocks, q_out, mode, dev_err};
-  return launch_append(a, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return rows <= 8 * sm_count() ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
 }
 
 extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t tokens, const int32_t *chunk_lens,
