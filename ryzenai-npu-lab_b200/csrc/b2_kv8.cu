@@ -1208,10 +1208,9 @@ struct __align__(16) PrefillTail {
   uint64_t raw[2][kPfRaw];       // codes landed (K, V)
   uint64_t full[2][kPfStages];   // operand written by its converter warp
   uint64_t empty[2][kPfStages];  // operand read by its product (commit)
-  uint64_t sbar[2];              // S_j computed (commit)
+  uint64_t sbar[2];              // S_j computed, and every product issued before it done (commit)
   uint64_t sfree[2];             // S_j read by the softmax threads
   uint64_t pready[2];            // P_j written by the softmax threads
-  uint64_t pfree[2];             // P_j read by its product (commit)
   uint64_t pvbar;                // P_j . V_j accumulated (commit per block)
   uint64_t obar;                 // every product done (one commit)
   uint32_t tmem;
@@ -1267,6 +1266,12 @@ __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0
   return true;
 }
 
+__device__ __forceinline__ float fmax3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
 __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const PrefillArgs a) {
   const int h = blockIdx.y;
   const int rank = static_cast<int>(blockIdx.z) / a.nsplit, split = static_cast<int>(blockIdx.z) - rank * a.nsplit;
@@ -1319,7 +1324,6 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       mbar_init(smem_u32(&tail->sbar[w]), 1);
       mbar_init(smem_u32(&tail->sfree[w]), 128);
       mbar_init(smem_u32(&tail->pready[w]), 128);
-      mbar_init(smem_u32(&tail->pfree[w]), 1);
     }
     mbar_init(smem_u32(&tail->pvbar), 1);
     mbar_init(smem_u32(&tail->obar), 1);
@@ -1474,7 +1478,6 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
         for (int ks = 0; ks < 4; ++ks)
           umma_f16_ta(tmem + 128, pt + 8 * ks, umma_desc(vt + 32 * ks, 16), kPfIdesc, (j > 0 || ks > 0) ? 1u : 0u);
         umma_commit(smem_u32(&tail->pvbar));
-        umma_commit(smem_u32(&tail->pfree[j & 1]));
         umma_commit(smem_u32(&tail->empty[1][s]));
         if (j + 2 < nblk) ok = issue_s(j + 2);
       }
@@ -1496,8 +1499,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     bool ok = true;
     // decided for the whole warp: the tensor memory accesses are warp-collective
     auto warp_wait = [&](uint32_t bar, uint32_t parity) -> bool {
-      const bool got = mbar_wait(bar, parity, a.wait_ns);
-      return !__any_sync(0xffffffffu, !got || tail->abort);
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.wait_ns));
     };
     // a warp whose rows are all past the chunk keeps step with the barriers only
     const bool active = __any_sync(0xffffffffu, row_ok);
@@ -1516,10 +1518,6 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       }
       if (!active) {
         mbar_arrive(smem_u32(&tail->sfree[j & 1]));
-        if (j >= 2 && !warp_wait(smem_u32(&tail->pfree[j & 1]), ((j >> 1) - 1) & 1)) {
-          ok = false;
-          break;
-        }
         mbar_arrive(smem_u32(&tail->pready[j & 1]));
         continue;
       }
@@ -1538,14 +1536,15 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
 #pragma unroll
         for (int c = 0; c < 64; ++c) sc[c] = c <= lim ? sc[c] : -INFINITY;
       }
-      float bm8[8];
+      float bm[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) bm8[e] = sc[e];
+      for (int e = 0; e < 4; ++e) bm[e] = fmaxf(sc[e], sc[e + 4]);
 #pragma unroll
-      for (int c = 8; c < 64; ++c) bm8[c & 7] = fmaxf(bm8[c & 7], sc[c]);
+      for (int c = 8; c < 64; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) bm[e] = fmax3(bm[e], sc[c + e], sc[c + 4 + e]);
       const float w = fmaxf(factor * ks, 1.2e-38f);  // not 0, which would make NaN of a masked score
-      const float top = fmaxf(fmaxf(fmaxf(bm8[0], bm8[1]), fmaxf(bm8[2], bm8[3])),
-                              fmaxf(fmaxf(bm8[4], bm8[5]), fmaxf(bm8[6], bm8[7]))) * w;
+      const float top = fmaxf(fmax3(bm[0], bm[1], bm[2]), bm[3]) * w;
       if (top > m + kSlack) {
         l *= ex2(m - top);
         m = top;
@@ -1606,11 +1605,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       } else {
         l = fmaf(sum, ex2(low), l);
       }
-      // into buffer j % 2 once the product that read it is done
-      if (j >= 2 && !warp_wait(smem_u32(&tail->pfree[j & 1]), ((j >> 1) - 1) & 1)) {
-        ok = false;
-        break;
-      }
+      // into buffer j % 2: P_{j-2} . V_{j-2}, which read it, was issued before S_j, so it is done
       tmem_st32(trow + 192 + 32 * (j & 1), pk);
       tmem_wait_st();
       tmem_fence_before();
@@ -1621,10 +1616,11 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       tail->abort = 1;
     } else if (warp_wait(smem_u32(&tail->obar), 0)) {
       tmem_fence_after();
+      const bool stop = __any_sync(0xffffffffu, tail->abort);
       float o[64];
       tmem_ld64(trow + 128, o);
       const float unit = ex2(mo - m);  // the output in units of 2^m, as the sum
-      if (tail->abort) {
+      if (stop) {
       } else if (pt.parts > 1) {
         PrefillState *st = a.parts + ((static_cast<int64_t>(b) * gridDim.x + tile) * kHkv + h) * a.nsplit + split;
         float4 *dst = reinterpret_cast<float4 *>(st->o[tid]);
