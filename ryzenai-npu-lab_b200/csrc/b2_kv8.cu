@@ -121,14 +121,15 @@ struct AppendArgs {
   int32_t *err;
 };
 
-constexpr int kMaxWindow = 64;   // rows whose runs start in one CTA: 8 or 64
+constexpr int kMaxWindow = 32;   // rows whose runs start in one CTA: 8 or 32, at most a warp's lanes
 constexpr int kNoSlot = -1;
-constexpr int kAppendThreads = 512;
+constexpr int kAppendWarps = 4;  // K and V of two heads
+constexpr int kAppendThreads = kAppendWarps * 32;
 
 // A run's rows of one head, K or V, per warp, and the places of the rows around.
 struct AppendShared {
-  uint16_t rows[kAppendThreads / 32][kBlock][kDim];
-  int slot[1 + kMaxWindow + kBlock], place[1 + kMaxWindow + kBlock];  // entry i: row row0 - 1 + i
+  uint16_t rows[kAppendWarps][kBlock][kDim];
+  int slot[1 + kMaxWindow + kBlock + 1], place[1 + kMaxWindow + kBlock + 1];  // entry i: row row0 - 1 + i
 };
 
 // Slot and RoPE position of a row; kNoSlot for a row to skip.
@@ -166,21 +167,21 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
   return blk * kBlock + static_cast<int>(pos % kBlock);
 }
 
-// One CTA per window of rows, warp = (KV head, K or V).  A run is a sequence of
+// One CTA per window of rows and pair of heads, warp = (KV head, K or V).  A run is a sequence of
 // adjacent rows that go to adjacent slots of one block; the warps of the window
 // that holds its first row quantise the whole run, each for its head, so a
 // block's scale is found and its codes are written by one warp alone, with no
-// atomics.  All of a run's loads are in flight together (up to 16 per lane; 8
-// lanes own one 64-wide head vector) on their way to shared memory, from where
-// norm and RoPE, the maximum and the codes are taken.  Codes leave in 16-byte
+// atomics.  A run's loads are copies to shared memory, all in flight together (up
+// to 16 per lane; 8 lanes own one 64-wide head vector) without registers, from
+// where norm and RoPE, the maximum and the codes are taken.  Codes leave in 16-byte
 // pieces: a lane takes 16 dims of a K row, or 16 tokens of two V dims, for which
 // shared memory is the transpose.
 //
-// Bound by latency for the few rows of a short prompt and by the reads of qkv
-// for long ones.  kWindow 8 spreads few rows over the SMs; 64 keeps the CTAs
-// that hold no run's start from outnumbering the others in long prompts.
+// Bound by latency: a run's loads, its codes, its stores.  kWindow 8 spreads few
+// rows over the SMs; 32 keeps the CTAs that hold no run's start from outnumbering
+// the others in long prompts.
 template <int kWindow>
-__global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
   extern __shared__ uint8_t smem_raw[];
   AppendShared &sh = *reinterpret_cast<AppendShared *>(smem_raw);
   const int row0 = static_cast<int>(blockIdx.x) * kWindow;
@@ -192,7 +193,7 @@ __global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const App
     int position = 0, flag = 0;
     sh.slot[i] = r >= 0 && r < a.rows ? row_place(a, static_cast<int>(r), position, flag) : kNoSlot;
     sh.place[i] = position;
-    if (i >= 1 && i <= kWindow) {
+    if (i >= 1 && i <= kWindow && blockIdx.y == 0) {
       if (sh.slot[i] >= 0 && (a.mode & B2_ROPE_QK) && (position < 0 || position >= a.rope_rows))
         flag |= B2_DEV_BAD_POSITION;
       if (flag) atomicOr(a.err, flag);
@@ -210,7 +211,8 @@ __global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const App
 
   if (a.q_out) {
     // four query heads of a row per pass, the passes of the window's rows over the warps
-    for (int p = warp; p < kWindow * (kHq / 4); p += kAppendThreads / 32) {
+    for (int p = static_cast<int>(blockIdx.y) * kAppendWarps + warp; p < kWindow * (kHq / 4);
+         p += static_cast<int>(gridDim.y) * kAppendWarps) {
       const int i = 1 + p / (kHq / 4), vec = 4 * (p % (kHq / 4)) + grp;
       if (sh.slot[i] < 0) continue;
       const int64_t r = row0 - 1 + i;
@@ -222,59 +224,60 @@ __global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const App
   }
   if (!(a.mode & B2_STORE_KV)) return;
 
-  const int h = warp >> 1;
+  const int h = static_cast<int>(blockIdx.y) * (kAppendWarps / 2) + (warp >> 1);
   const bool is_v = warp & 1;
   uint16_t(*rows)[kDim] = sh.rows[warp];
-  for (int i0 = 1; i0 <= kWindow; ++i0) {
-    const int s0 = sh.slot[i0];
-    if (s0 < 0) continue;
-    const int blk = s0 / kBlock, r0 = s0 % kBlock, prev = sh.slot[i0 - 1];
-    if (prev >= 0 && prev + 1 == s0 && r0 != 0) continue;  // inside a run
-    int n = 1;
-    while (r0 + n < kBlock && sh.slot[i0 + n] == s0 + n) ++n;
+  // rows of the window that start a run: valid, and not the slot behind the row before in the same block
+  const int here = lane < kWindow ? sh.slot[1 + lane] : kNoSlot, before = lane < kWindow ? sh.slot[lane] : kNoSlot;
+  uint32_t starts = __ballot_sync(0xffffffffu, here >= 0 && (before < 0 || before + 1 != here || here % kBlock == 0));
+  for (; starts; starts &= starts - 1) {
+    const int i0 = __ffs(starts), s0 = sh.slot[i0];
+    const int blk = s0 / kBlock, r0 = s0 % kBlock;
+    // rows that follow: 1 + lane, 33 + lane behind the first
+    const uint32_t m0 = __ballot_sync(0xffffffffu, r0 + 1 + lane < kBlock && sh.slot[i0 + 1 + lane] == s0 + 1 + lane);
+    const uint32_t m1 = __ballot_sync(0xffffffffu, r0 + 33 + lane < kBlock && sh.slot[i0 + 33 + lane] == s0 + 33 + lane);
+    const int n = 1 + (m0 != 0xffffffffu ? __ffs(~m0) - 1 : 32 + __ffs(~m1) - 1);  // lane 31 of m1 would be row 64
     const uint16_t *src = a.qkv + (static_cast<int64_t>(row0) - 1 + i0 + grp) * a.row_stride +
                           (kHq + (is_v ? kHkv : 0) + h) * kDim + j * 8;
-    uint4 w[kBlock / 4];
-#pragma unroll
-    for (int i = 0; i < kBlock / 4; ++i)
-      if (4 * i + grp < n) w[i] = __ldg(reinterpret_cast<const uint4 *>(src + 4 * i * a.row_stride));
-    float amax = 0.f;
-    if (is_v || !(norm || rope)) {
-#pragma unroll
-      for (int i = 0; i < kBlock / 4; ++i) {
-        if (4 * i + grp >= n) continue;
-        float x[8];
-        unpack8(w[i], x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, limited_abs(x[e]));
-        *reinterpret_cast<uint4 *>(&rows[4 * i + grp][8 * j]) = w[i];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kBlock / 4; ++i)
-        if (4 * i + grp < n) *reinterpret_cast<uint4 *>(&rows[4 * i + grp][8 * j]) = w[i];
-      for (int i = 0; i < n; i += 4) {
-        const bool live = i + grp < n;
-        float x[8];
-        unpack8(live ? *reinterpret_cast<const uint4 *>(&rows[i + grp][8 * j]) : make_uint4(0u, 0u, 0u, 0u), x);
-        turn(x, live ? i0 + i + grp : 0, a.gamma_k);
-        if (!live) continue;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, limited_abs(x[e]));
-        *reinterpret_cast<uint4 *>(&rows[i + grp][8 * j]) = pack8(x);
-      }
-    }
+    const uint32_t dst = smem_u32(&rows[grp][8 * j]);
+    for (int i = 0; i < n; i += 4)
+      if (i + grp < n)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * kDim * 2), "l"(src + i * a.row_stride)
+                     : "memory");
     const int64_t id = static_cast<int64_t>(blk) * kHkv + h;
     float *sp = (is_v ? a.v_scale : a.k_scale) + id;
     uint8_t *codes = (is_v ? a.v_pool : a.k_pool) + id * kTile;
     const float old = r0 > 0 ? *sp : 0.f;
-    const float s = fmaxf(scale_for(warp_max(amax)), old), inv = 1.0f / s;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    const bool turned = !is_v && (norm || rope);
+    float amax = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; i += 4) {
+      const bool live = i + grp < n;
+      float x[8];
+      unpack8(live ? *reinterpret_cast<const uint4 *>(&rows[i + grp][8 * j]) : make_uint4(0u, 0u, 0u, 0u), x);
+      if (turned) {
+        turn(x, live ? i0 + i + grp : 0, a.gamma_k);
+        if (live) *reinterpret_cast<uint4 *>(&rows[i + grp][8 * j]) = pack8(x);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, live ? limited_abs(x[e]) : 0.f);
+    }
+    amax = warp_max(amax);
+    const float s = fmaxf(scale_for(amax), old), inv = 1.0f / s;
+    const bool finite = amax < kBf16Max;  // no value to limit
     const bool raise = r0 > 0 && s > old;  // the rows in front of the run move to the larger scale
     const float ratio = raise ? old / s : 1.f;
     __syncwarp();
     if (lane == 0) *sp = s;
-    auto code = [&](uint32_t two) {  // two bf16 as two codes
-      return e4m3x2(limited(__uint_as_float(two << 16)) * inv, limited(__uint_as_float(two & 0xffff0000u)) * inv);
+    auto code = [&](uint32_t two) -> uint32_t {  // two bf16 as two codes
+      float x = __uint_as_float(two << 16), y = __uint_as_float(two & 0xffff0000u);
+      if (!finite) {
+        x = limited(x);
+        y = limited(y);
+      }
+      return e4m3x2(x * inv, y * inv);
     };
     if (!is_v) {
       // 4 lanes per row, 16 dims each
@@ -296,16 +299,28 @@ __global__ void __launch_bounds__(kAppendThreads, 1) kv8_append_kernel(const App
       for (int q = first; q <= last; ++q) {
         uint4 *p0 = reinterpret_cast<uint4 *>(codes + 2 * lane * kBlock) + q, *p1 = p0 + kBlock / 16;
         const int lo = r0 - 16 * q, hi = r0 + n - 16 * q;  // rows of the run in this piece: [lo, hi)
-        uint32_t u[4] = {0u, 0u, 0u, 0u}, v[4] = {0u, 0u, 0u, 0u};
-        if (lo > 0 || hi < 16) {
-          uint4 x = *p0, y = *p1;
-          if (raise && lo > 0) {
-            x = rescale16(x, ratio, lo);
-            y = rescale16(y, ratio, lo);
+        uint32_t u[4], v[4];
+        if (lo <= 0 && hi >= 16) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            uint32_t c[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[e] = code(*reinterpret_cast<const uint32_t *>(&rows[i + e - lo][2 * lane]));
+            const uint32_t x = __byte_perm(c[0], c[1], 0x5410), y = __byte_perm(c[2], c[3], 0x5410);
+            u[i >> 2] = __byte_perm(x, y, 0x6420);
+            v[i >> 2] = __byte_perm(x, y, 0x7531);
           }
-          u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
-          v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
+          *p0 = make_uint4(u[0], u[1], u[2], u[3]);
+          *p1 = make_uint4(v[0], v[1], v[2], v[3]);
+          continue;
         }
+        uint4 x = *p0, y = *p1;
+        if (raise && lo > 0) {
+          x = rescale16(x, ratio, lo);
+          y = rescale16(y, ratio, lo);
+        }
+        u[0] = x.x; u[1] = x.y; u[2] = x.z; u[3] = x.w;
+        v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           if (i < lo || i >= hi) continue;
@@ -1790,7 +1805,7 @@ int launch_append(const AppendArgs &a, cudaStream_t st) {
     done[dev] = true;
   }
   const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(a.rows) + kWindow - 1) / kWindow);
-  kv8_append_kernel<kWindow><<<grid, kAppendThreads, sizeof(AppendShared), st>>>(a);
+  kv8_append_kernel<kWindow><<<dim3(grid, 2 * kHkv / kAppendWarps), kAppendThreads, sizeof(AppendShared), st>>>(a);
   return launched(cudaSuccess, "kv8_append_kernel");
 }
 
@@ -1830,7 +1845,7 @@ extern "C" int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t ro
                max_blocks_per_seq, gamma_q, gamma_k, eps, rope_cos, rope_sin, rope_rows, k_pool, v_pool,
                k_scale, v_scale, num_blocks, q_out, mode, dev_err};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return rows <= 8 * sm_count() ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
+  return rows <= 1024 ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
 }
 
 extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t tokens, const int32_t *chunk_lens,
