@@ -1,7 +1,8 @@
 // Block tables and slot maps built on the GPU (include/b2_tables.h):
 //
 //   extend_kernel   blocks for new tokens off the end of the free list, in
-//                   request order: prefix sums of rows and of needed blocks
+//                   request order: prefix sums of rows and of needed blocks;
+//                   for few rows their slots and positions too
 //   slot_kernel     slot and position of every new token's row
 //   release_kernel  blocks of finished requests back to the free list
 //
@@ -21,7 +22,10 @@ namespace {
 
 constexpr int kBlock = 64;
 constexpr int kScanThreads = 1024;
-constexpr int kSlotThreads = 256;
+constexpr int kSlotThreads = 128;
+constexpr int kRowsHere = kScanThreads;  // rows that extend_kernel writes itself, one per thread
+constexpr int kRowsWide = 1 << 16;       // rows from which a thread of slot_kernel takes 8 instead of 1
+constexpr int kFewBlocks = 16;           // blocks that a thread fetches for its own request
 constexpr int32_t kMaxTableWidth = (1 << 25) - 1;  // width x 64 tokens stay an int32
 constexpr int32_t kMaxPoolBlocks = (1 << 22) - 1;
 
@@ -61,82 +65,6 @@ __device__ __forceinline__ int last_at_or_below(const T *start, int n, T x) {
   return lo;
 }
 
-struct ExtendArgs {
-  int32_t *tables;
-  int max_blocks;
-  const int32_t *held, *free_list;
-  int num_blocks;
-  const int32_t *free_count, *past, *fresh;
-  int batch;
-  int32_t *held_out, *count_out, *granted, *row_start;
-  int rows, tokens;
-  int32_t *err;
-};
-
-// One CTA walks the requests, kScanThreads at a time: two prefix sums (rows,
-// needed blocks), then the new table entries of the chunk spread over all
-// threads (an entry finds its request by bisection of the chunk's sums), so
-// one request of many blocks costs no more than many of one.
-__global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a) {
-  __shared__ int64_t warp_sum[kScanThreads / 32];
-  __shared__ int64_t first[kScanThreads];  // exclusive sums of the blocks taken in this chunk
-  __shared__ int32_t from[kScanThreads];   // blocks held before
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  int64_t count = a.free_count[0];
-  int flag = 0;
-  if (count < 0 || count > a.num_blocks) {
-    flag = B2_DEV_BAD_LENGTH;
-    count = count < 0 ? 0 : a.num_blocks;
-  }
-  int64_t rows_before = 0, need_before = 0, taken = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kScanThreads) {
-    const int b = b0 + static_cast<int>(threadIdx.x);
-    const bool in = b < a.batch;
-    const int past = in ? a.past[b] : 0, fresh = in ? a.fresh[b] : 0, held = in ? a.held[b] : 0;
-    const int64_t upto = static_cast<int64_t>(past) + fresh;
-    bool bad = past < 0 || fresh < 0 || held < 0 || held > a.max_blocks ||
-               upto > static_cast<int64_t>(a.max_blocks) * kBlock || (a.tokens > 0 && fresh > a.tokens);
-    int64_t total = 0;
-    int64_t start = static_cast<int64_t>(b) * a.tokens;
-    if (a.tokens == 0) {
-      const int64_t n = fresh > 0 ? fresh : 0;
-      start = rows_before + scan_exclusive(n, warp_sum, total);
-      rows_before += total;
-      if (n > 0 && start + n > a.rows) bad = true;
-    }
-    if (bad) flag = B2_DEV_BAD_LENGTH;
-    const int64_t blocks = (upto + kBlock - 1) / kBlock;
-    const int64_t need = in && !bad && blocks > held ? blocks - held : 0;
-    const int64_t pre = need_before + scan_exclusive(need, warp_sum, total);
-    need_before += total;
-    const bool ok = !bad && (need == 0 || pre + need <= count);
-    const int64_t take = ok ? need : 0;
-    int64_t chunk = 0;
-    const int64_t pos = scan_exclusive(take, warp_sum, chunk);
-    first[threadIdx.x] = pos;
-    from[threadIdx.x] = held;
-    __syncthreads();
-    for (int64_t e = threadIdx.x; e < chunk; e += kScanThreads) {
-      const int i = last_at_or_below<int64_t>(first, kScanThreads, e);
-      int id = a.free_list[count - 1 - (taken + e)];
-      if (id < 0 || id >= a.num_blocks) {
-        flag |= B2_DEV_BAD_BLOCK;
-        id = -1;
-      }
-      a.tables[static_cast<int64_t>(b0 + i) * a.max_blocks + from[i] + (e - first[i])] = id;
-    }
-    taken += chunk;
-    if (in) {
-      a.held_out[b] = held + static_cast<int32_t>(take);
-      a.granted[b] = ok ? fresh : 0;
-      a.row_start[b] = static_cast<int32_t>(start < a.rows ? start : a.rows);
-    }
-    __syncthreads();
-  }
-  if (flag) atomicOr(a.err, flag);
-  if (threadIdx.x == 0) a.count_out[0] = static_cast<int32_t>(count - taken);
-}
-
 struct SlotArgs {
   const int32_t *tables;
   int max_blocks, num_blocks;
@@ -147,36 +75,223 @@ struct SlotArgs {
   int32_t *err;  // NULL: faults were reported before
 };
 
-// One thread per row; packed rows find their request by bisection.
+// Rows r0 .. r0 + kSlotRows - 1, ascending from request b on (the last one that
+// starts at or before r0): eight rows share the search for their request and
+// leave as 16-byte stores; one row per thread keeps few rows' loads parallel.
+template <bool kPadded, int kSlotRows>
+__device__ __forceinline__ void write_rows(const SlotArgs &a, int64_t r0, int b) {
+  int slot[kSlotRows], position[kSlotRows];
+  int64_t start = 0;
+  int past = 0, fresh = 0, flag = 0, held_blk = -1, blk = -1;
+  bool granted = false;
+  auto request = [&]() {
+    const bool in = b >= 0 && b < a.batch;
+    start = !in ? 0 : (kPadded ? static_cast<int64_t>(b) * a.tokens : a.row_start[b]);
+    past = in ? a.past[b] : 0;
+    fresh = in ? a.fresh[b] : 0;
+    granted = in && (!a.granted || a.granted[b] > 0);
+    held_blk = -1;
+  };
+  request();
+#pragma unroll
+  for (int i = 0; i < kSlotRows; ++i) {
+    const int64_t r = r0 + i;
+    slot[i] = -1;
+    position[i] = 0;
+    if (r >= a.rows) continue;
+    if (kPadded) {
+      if (r - start >= a.tokens) {
+        ++b;
+        request();
+      }
+    } else {
+      bool moved = false;
+      while (b + 1 < a.batch && a.row_start[b + 1] <= r) {
+        ++b;
+        moved = true;
+      }
+      if (moved) request();
+    }
+    const int64_t t = r - start;
+    if (b < 0 || b >= a.batch || t >= fresh) continue;
+    const int64_t pos = past + t;
+    position[i] = static_cast<int>(pos);
+    if (!granted) continue;
+    if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) {
+      flag |= B2_DEV_BAD_LENGTH;
+      continue;
+    }
+    const int logical = static_cast<int>(pos / kBlock);
+    if (logical != held_blk) {
+      blk = a.tables[static_cast<int64_t>(b) * a.max_blocks + logical];
+      held_blk = logical;
+    }
+    if (blk < 0 || blk >= a.num_blocks) flag |= B2_DEV_BAD_BLOCK;
+    else slot[i] = blk * kBlock + static_cast<int>(pos % kBlock);
+  }
+  if (flag && a.err) atomicOr(a.err, flag);
+  const bool wide = kSlotRows >= 4 && r0 + kSlotRows <= a.rows &&
+                    ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0;
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i + 3 < kSlotRows; i += 4) {
+      *reinterpret_cast<int4 *>(a.slots + r0 + i) = make_int4(slot[i], slot[i + 1], slot[i + 2], slot[i + 3]);
+      *reinterpret_cast<int4 *>(a.positions + r0 + i) =
+          make_int4(position[i], position[i + 1], position[i + 2], position[i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kSlotRows; ++i)
+      if (r0 + i < a.rows) {
+        a.slots[r0 + i] = slot[i];
+        a.positions[r0 + i] = position[i];
+      }
+  }
+}
+
+// Rows r0 .. of any request.
+template <int kSlotRows>
+__device__ __forceinline__ void find_and_write_rows(const SlotArgs &a, int64_t r0) {
+  if (!a.row_start) write_rows<true, kSlotRows>(a, r0, static_cast<int>(r0 / a.tokens));
+  else write_rows<false, kSlotRows>(a, r0, last_at_or_below<int32_t>(a.row_start, a.batch, static_cast<int32_t>(r0)));
+}
+
+struct ExtendArgs {
+  int32_t *tables;
+  int max_blocks;
+  const int32_t *held, *free_list;
+  int num_blocks;
+  const int32_t *free_count, *past, *fresh;
+  int batch;
+  int32_t *held_out, *count_out, *granted, *row_start;
+  int rows, tokens;
+  int32_t *err;
+  SlotArgs slots;  // rows > 0: to be written here
+};
+
+// One CTA walks the requests, kPer per thread and kScanThreads * kPer at a time:
+// prefix sums of their rows and needed blocks, then the new table entries of the
+// chunk spread over all threads (an entry finds its request by bisection of the
+// chunk's sums), so one request of many blocks costs no more than many of one.
+// The requests that get blocks are the first ones that need any, so their sums
+// of needed blocks are their places on the free list.
+template <int kPer>
+__global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a) {
+  __shared__ int64_t warp_sum[kScanThreads / 32];
+  __shared__ int32_t first[kScanThreads * kPer];  // exclusive sums of the blocks needed in this chunk
+  __shared__ int32_t from[kScanThreads * kPer];   // blocks held before
+  __shared__ unsigned long long taken_here;       // blocks given to the chunk's requests
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int64_t count = a.free_count[0];
+  int flag = 0;
+  if (count < 0 || count > a.num_blocks) {
+    flag = B2_DEV_BAD_LENGTH;
+    count = count < 0 ? 0 : a.num_blocks;
+  }
+  int64_t rows_before = 0, need_before = 0, taken = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kScanThreads * kPer) {
+    const int i0 = static_cast<int>(threadIdx.x) * kPer;
+    int past[kPer], fresh[kPer], held[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int b = b0 + i0 + e;
+      past[e] = b < a.batch ? a.past[b] : 0;
+      fresh[e] = b < a.batch ? a.fresh[b] : 0;
+      held[e] = b < a.batch ? a.held[b] : 0;
+    }
+    if (threadIdx.x == 0) taken_here = 0;
+    int64_t total = 0, start[kPer], need[kPer], mine = 0;
+    if (a.tokens == 0) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) mine += fresh[e] > 0 ? fresh[e] : 0;
+      int64_t at = rows_before + scan_exclusive(mine, warp_sum, total);
+      rows_before += total;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        start[e] = at;
+        at += fresh[e] > 0 ? fresh[e] : 0;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) start[e] = static_cast<int64_t>(b0 + i0 + e) * a.tokens;
+    }
+    bool bad[kPer];
+    mine = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int64_t upto = static_cast<int64_t>(past[e]) + fresh[e];
+      bad[e] = past[e] < 0 || fresh[e] < 0 || held[e] < 0 || held[e] > a.max_blocks ||
+               upto > static_cast<int64_t>(a.max_blocks) * kBlock || (a.tokens > 0 && fresh[e] > a.tokens) ||
+               (a.tokens == 0 && fresh[e] > 0 && start[e] + fresh[e] > a.rows);
+      if (bad[e]) flag |= B2_DEV_BAD_LENGTH;
+      const int64_t blocks = (upto + kBlock - 1) / kBlock;
+      need[e] = !bad[e] && blocks > held[e] ? blocks - held[e] : 0;
+      mine += need[e];
+    }
+    int64_t pre = scan_exclusive(mine, warp_sum, total);
+    int64_t end = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int b = b0 + i0 + e;
+      first[i0 + e] = pre < 0x7fffffff ? static_cast<int32_t>(pre) : 0x7fffffff;  // (no list is that long)
+      from[i0 + e] = held[e];
+      const bool ok = !bad[e] && (need[e] == 0 || need_before + pre + need[e] <= count);
+      pre += need[e];
+      if (ok && need[e] > 0) end = pre;
+      if (b < a.batch) {
+        a.held_out[b] = held[e] + (ok ? static_cast<int32_t>(need[e]) : 0);
+        a.granted[b] = ok ? fresh[e] : 0;
+        a.row_start[b] = static_cast<int32_t>(start[e] < a.rows ? start[e] : a.rows);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+      const int64_t u = __shfl_xor_sync(0xffffffffu, end, off);
+      end = u > end ? u : end;
+    }
+    if ((threadIdx.x & 31) == 0 && end > 0) atomicMax(&taken_here, static_cast<unsigned long long>(end));
+    __syncthreads();
+    const int chunk = static_cast<int>(taken_here);
+    auto block = [&](int64_t e) {  // the e-th block of the chunk
+      const int id = a.free_list[count - 1 - (need_before + e)];
+      if (id >= 0 && id < a.num_blocks) return id;
+      flag |= B2_DEV_BAD_BLOCK;
+      return -1;
+    };
+    // few blocks per request: its own thread fetches them; else the entries are
+    // spread over all threads
+    bool few = true;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) few = few && need[e] <= kFewBlocks;
+    if (__syncthreads_and(few)) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int at = first[i0 + e];
+        int32_t *entry = a.tables + static_cast<int64_t>(b0 + i0 + e) * a.max_blocks + held[e];
+#pragma unroll 4
+        for (int i = 0; i < static_cast<int>(need[e]) && at + i < chunk; ++i) entry[i] = block(at + i);
+      }
+    } else
+    for (int e = threadIdx.x; e < chunk; e += kScanThreads) {
+      const int i = last_at_or_below<int32_t>(first, kScanThreads * kPer, e);
+      a.tables[static_cast<int64_t>(b0 + i) * a.max_blocks + from[i] + (e - first[i])] = block(e);
+    }
+    taken += chunk;
+    need_before += total;  // with what was refused: nobody behind a refused request gets a block
+    __syncthreads();
+  }
+  if (flag) atomicOr(a.err, flag);
+  __syncthreads();  // every thread has read the old count, and sees the starts, grants and entries
+  if (threadIdx.x == 0) a.count_out[0] = static_cast<int32_t>(count - taken);
+  if (a.slots.rows > 0)
+    for (int64_t r = threadIdx.x; r < a.slots.rows; r += kScanThreads) find_and_write_rows<1>(a.slots, r);
+}
+
+template <int kSlotRows>
 __global__ void __launch_bounds__(kSlotThreads) slot_kernel(const SlotArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x;
-  if (r >= a.rows) return;
-  int b;
-  if (a.tokens > 0 && !a.row_start) b = static_cast<int>(r / a.tokens);
-  else b = last_at_or_below<int32_t>(a.row_start, a.batch, static_cast<int32_t>(r));
-  int slot = -1, position = 0;
-  if (b >= 0 && b < a.batch) {
-    const int64_t start = a.row_start ? a.row_start[b] : static_cast<int64_t>(b) * a.tokens;
-    const int64_t t = r - start;
-    if (t < a.fresh[b]) {
-      const int64_t pos = a.past[b] + t;
-      position = static_cast<int>(pos);
-      int flag = 0;
-      if (!a.granted || a.granted[b] > 0) {
-        if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) {
-          flag = B2_DEV_BAD_LENGTH;
-        } else {
-          const int blk = a.tables[static_cast<int64_t>(b) * a.max_blocks + pos / kBlock];
-          if (blk < 0 || blk >= a.num_blocks) flag = B2_DEV_BAD_BLOCK;
-          else slot = blk * kBlock + static_cast<int>(pos % kBlock);
-        }
-      }
-      if (flag && a.err) atomicOr(a.err, flag);
-    }
-  }
-  a.slots[r] = slot;
-  a.positions[r] = position;
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x) * kSlotRows;
+  if (r0 < a.rows) find_and_write_rows<kSlotRows>(a, r0);
 }
 
 struct ReleaseArgs {
@@ -242,7 +357,9 @@ int launched(cudaError_t e, const char *what) {
 int launch_slots(const SlotArgs &a, bool dependent, cudaStream_t st) {
   if (a.rows == 0) return b2_clear_error();
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(a.rows) + kSlotThreads - 1) / kSlotThreads));
+  const bool wide = a.rows >= kRowsWide;
+  const int per = kSlotThreads * (wide ? 8 : 1);
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(a.rows) + per - 1) / per));
   cfg.blockDim = dim3(kSlotThreads);
   cfg.stream = st;
   cudaLaunchAttribute pdl[1];
@@ -250,7 +367,8 @@ int launch_slots(const SlotArgs &a, bool dependent, cudaStream_t st) {
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl;
   cfg.numAttrs = dependent ? 1 : 0;
-  return launched(cudaLaunchKernelEx(&cfg, slot_kernel, a), "slot_kernel");
+  return launched(wide ? cudaLaunchKernelEx(&cfg, slot_kernel<8>, a) : cudaLaunchKernelEx(&cfg, slot_kernel<1>, a),
+                  "slot_kernel");
 }
 
 int check_sizes(int32_t max_blocks, int32_t num_blocks, int32_t batch, int32_t rows, int32_t tokens) {
@@ -278,14 +396,17 @@ extern "C" int b2_tables_extend(int32_t *block_tables, int32_t max_blocks_per_se
       (rows > 0 && (!slots || !positions)))
     return fail(B2_ERR_ARG, "b2_tables_extend: null pointer argument");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  ExtendArgs a{block_tables, max_blocks_per_seq, held, free_list, num_blocks, free_count, past_lens, new_lens, batch,
-               held_out, free_count_out, granted, row_start, rows, tokens_per_seq, dev_err};
-  extend_kernel<<<1, kScanThreads, 0, st>>>(a);
-  const int lrc = launched(cudaSuccess, "extend_kernel");
-  if (lrc) return lrc;
   SlotArgs s{block_tables, max_blocks_per_seq, num_blocks, past_lens, new_lens, granted,
              tokens_per_seq > 0 ? nullptr : row_start, batch, slots, positions, rows, tokens_per_seq, nullptr};
-  return launch_slots(s, true, st);
+  ExtendArgs a{block_tables, max_blocks_per_seq, held, free_list, num_blocks, free_count, past_lens, new_lens, batch,
+               held_out, free_count_out, granted, row_start, rows, tokens_per_seq, dev_err, s};
+  // few rows are written by the CTA that has the sums: one launch
+  const bool here = rows <= kRowsHere;
+  if (!here) a.slots.rows = 0;
+  if (batch <= kScanThreads) extend_kernel<1><<<1, kScanThreads, 0, st>>>(a);
+  else extend_kernel<4><<<1, kScanThreads, 0, st>>>(a);
+  const int lrc = launched(cudaSuccess, "extend_kernel");
+  return lrc || here ? lrc : launch_slots(s, true, st);
 }
 
 extern "C" int b2_slot_map(const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t num_blocks,
