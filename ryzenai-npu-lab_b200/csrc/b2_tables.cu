@@ -25,6 +25,7 @@ constexpr int kScanThreads = 1024;
 constexpr int kSlotThreads = 128;
 constexpr int kRowsHere = kScanThreads;  // rows that extend_kernel writes itself, one per thread
 constexpr int kRowsWide = 1 << 16;       // rows from which a thread of slot_kernel takes 8 instead of 1
+constexpr int kExtendCtas = 8;           // cluster of extend_kernel for more than kScanThreads requests
 constexpr int kFewBlocks = 16;           // blocks that a thread fetches for its own request
 constexpr int32_t kMaxTableWidth = (1 << 25) - 1;  // width x 64 tokens stay an int32
 constexpr int32_t kMaxPoolBlocks = (1 << 22) - 1;
@@ -175,13 +176,20 @@ struct ExtendArgs {
 // chunk's sums), so one request of many blocks costs no more than many of one.
 // The requests that get blocks are the first ones that need any, so their sums
 // of needed blocks are their places on the free list.
-template <int kPer>
+//
+// Many requests' entries are scattered 4-byte stores, about one per clock of an
+// SM (16 000 entries: 11 of 20 us), so a cluster of kCtas CTAs computes the sums
+// alike and shares the stores.  held_out and free_count_out may be the inputs: a
+// cluster barrier stands between each chunk's loads and its stores.
+template <int kPer, int kCtas>
 __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a) {
   __shared__ int64_t warp_sum[kScanThreads / 32];
   __shared__ int32_t first[kScanThreads * kPer];  // exclusive sums of the blocks needed in this chunk
   __shared__ int32_t from[kScanThreads * kPer];   // blocks held before
   __shared__ unsigned long long taken_here;       // blocks given to the chunk's requests
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int cta = static_cast<int>(blockIdx.x);                           // of the cluster
+  const bool own = static_cast<int>(threadIdx.x) / (kScanThreads / kCtas) == cta;  // this CTA stores for this thread's requests
   int64_t count = a.free_count[0];
   int flag = 0;
   if (count < 0 || count > a.num_blocks) {
@@ -200,6 +208,10 @@ __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a
       held[e] = b < a.batch ? a.held[b] : 0;
     }
     if (threadIdx.x == 0) taken_here = 0;
+    if (kCtas > 1) {
+      asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    }
     int64_t total = 0, start[kPer], need[kPer], mine = 0;
     if (a.tokens == 0) {
 #pragma unroll
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a
       const bool ok = !bad[e] && (need[e] == 0 || need_before + pre + need[e] <= count);
       pre += need[e];
       if (ok && need[e] > 0) end = pre;
-      if (b < a.batch) {
+      if (own && b < a.batch) {
         a.held_out[b] = held[e] + (ok ? static_cast<int32_t>(need[e]) : 0);
         a.granted[b] = ok ? fresh[e] : 0;
         a.row_start[b] = static_cast<int32_t>(start[e] < a.rows ? start[e] : a.rows);
@@ -265,14 +277,14 @@ __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a
     for (int e = 0; e < kPer; ++e) few = few && need[e] <= kFewBlocks;
     if (__syncthreads_and(few)) {
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
+      for (int e = 0; e < kPer && own; ++e) {
         const int at = first[i0 + e];
         int32_t *entry = a.tables + static_cast<int64_t>(b0 + i0 + e) * a.max_blocks + held[e];
 #pragma unroll 4
         for (int i = 0; i < static_cast<int>(need[e]) && at + i < chunk; ++i) entry[i] = block(at + i);
       }
     } else
-    for (int e = threadIdx.x; e < chunk; e += kScanThreads) {
+    for (int e = cta * kScanThreads + threadIdx.x; e < chunk; e += kCtas * kScanThreads) {
       const int i = last_at_or_below<int32_t>(first, kScanThreads * kPer, e);
       a.tables[static_cast<int64_t>(b0 + i) * a.max_blocks + from[i] + (e - first[i])] = block(e);
     }
@@ -282,8 +294,8 @@ __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a
   }
   if (flag) atomicOr(a.err, flag);
   __syncthreads();  // every thread has read the old count, and sees the starts, grants and entries
-  if (threadIdx.x == 0) a.count_out[0] = static_cast<int32_t>(count - taken);
-  if (a.slots.rows > 0)
+  if (cta == 0 && threadIdx.x == 0) a.count_out[0] = static_cast<int32_t>(count - taken);
+  if (kCtas == 1 && a.slots.rows > 0)
     for (int64_t r = threadIdx.x; r < a.slots.rows; r += kScanThreads) find_and_write_rows<1>(a.slots, r);
 }
 
@@ -401,11 +413,22 @@ extern "C" int b2_tables_extend(int32_t *block_tables, int32_t max_blocks_per_se
   ExtendArgs a{block_tables, max_blocks_per_seq, held, free_list, num_blocks, free_count, past_lens, new_lens, batch,
                held_out, free_count_out, granted, row_start, rows, tokens_per_seq, dev_err, s};
   // few rows are written by the CTA that has the sums: one launch
-  const bool here = rows <= kRowsHere;
+  const bool one = batch <= kScanThreads, here = one && rows <= kRowsHere;
   if (!here) a.slots.rows = 0;
-  if (batch <= kScanThreads) extend_kernel<1><<<1, kScanThreads, 0, st>>>(a);
-  else extend_kernel<4><<<1, kScanThreads, 0, st>>>(a);
-  const int lrc = launched(cudaSuccess, "extend_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(one ? 1 : kExtendCtas);
+  cfg.blockDim = dim3(kScanThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = kExtendCtas;
+  cluster[0].val.clusterDim.y = 1;
+  cluster[0].val.clusterDim.z = 1;
+  cfg.attrs = cluster;
+  cfg.numAttrs = one ? 0 : 1;
+  const int lrc = launched(one ? cudaLaunchKernelEx(&cfg, extend_kernel<1, 1>, a)
+                               : cudaLaunchKernelEx(&cfg, extend_kernel<4, kExtendCtas>, a),
+                           "extend_kernel");
   return lrc || here ? lrc : launch_slots(s, true, st);
 }
 
