@@ -645,6 +645,30 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
   // tiles of 32 positions: one per lane, those not issued yet in `left`
   int base = w0, entry = look(w0 + lane, true), entry_next = kNoTile, issued = 0;
   uint32_t left = __ballot_sync(0xffffffffu, entry != kNoTile);
+  // the segment after (b, h): its sequence
+  auto following = [&](int sb) {
+    do ++sb; while (sb < a.batch && sh.pos[sb + 1] == sh.pos[sb]);
+    return sb;
+  };
+  if (blk >= nblk && ++h == kHkv) {  // starts behind a segment's last tile
+    h = 0;
+    b = following(b);
+  }
+  // head vectors of the segment's new tokens, bf16: q (lanes 0-15), k (16-23) and
+  // v (24-31), and those of the next segment on their way
+  uint4 fresh[kT], fresh_next[kT];
+  auto fetch = [&](int sb, int head) {
+    const int vec = grp < 2 ? 2 * head + grp : (grp == 2 ? kHq + head : kHq + kHkv + head);
+    const uint16_t *p = a.qkv + static_cast<int64_t>(sb) * a.tokens * a.row_stride + vec * kDim + j * 8;
+#pragma unroll
+    for (int i = 0; i < kT; ++i)
+      if (i < sh.fresh[sb]) fresh_next[i] = __ldg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
+  };
+  if (blk >= nblk) blk = 0;
+  if (b < a.batch && w0 < w1) {
+    nblk = (sh.pos[b + 1] - sh.pos[b]) / kHkv - kSegmentCost;
+    fetch(b, h);  // ahead of the tiles, behind which it would queue
+  }
   bool looked = false;  // entry_next is the next 32 positions
   float2 scales[kStages];  // k and v scale of the tiles in flight, the next one's first
   auto issue = [&]() {
@@ -683,34 +707,10 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
   constexpr int kSets = Shared::kSets;
   uint32_t bq[4][2];
   float o[4][4], m[kSets], mo[kSets], l[kSets], factor[kSets];
-  // head vectors of the segment's new tokens, bf16: q (lanes 0-15), k (16-23) and
-  // v (24-31), and those of the next segment on their way
-  uint4 fresh[kT], fresh_next[kT];
-  auto fetch = [&](int sb, int head) {
-    const int vec = grp < 2 ? 2 * head + grp : (grp == 2 ? kHq + head : kHq + kHkv + head);
-    const uint16_t *p = a.qkv + static_cast<int64_t>(sb) * a.tokens * a.row_stride + vec * kDim + j * 8;
-#pragma unroll
-    for (int i = 0; i < kT; ++i)
-      if (i < sh.fresh[sb]) fresh_next[i] = __ldg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
-  };
-  // the segment after (b, h): its sequence
-  auto following = [&](int sb) {
-    do ++sb; while (sb < a.batch && sh.pos[sb + 1] == sh.pos[sb]);
-    return sb;
-  };
-  if (blk >= nblk && ++h == kHkv) {  // starts behind a segment's last tile
-    h = 0;
-    b = following(b);
-  }
   bool begin = true, from_start = false;  // the next tile is the segment's first in this warp, .. of all
   int past = 0, ntok = 0;
   bool ok = true;
-  if (issued > 0) {
-    if (blk >= nblk) blk = 0;
-    nblk = (sh.pos[b + 1] - sh.pos[b]) / kHkv - kSegmentCost;
-    from_start = blk == 0;
-    fetch(b, h);
-  }
+  from_start = blk == 0;
   for (int k = 0; k < issued; ++k) {
     const int s = k % kStages;
     if (begin) {
