@@ -167,19 +167,20 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
   return blk * kBlock + static_cast<int>(pos % kBlock);
 }
 
-// One CTA per window of rows and pair of heads, warp = (KV head, K or V).  A run is a sequence of
-// adjacent rows that go to adjacent slots of one block; the warps of the window
-// that holds its first row quantise the whole run, each for its head, so a
-// block's scale is found and its codes are written by one warp alone, with no
-// atomics.  A run's loads are copies to shared memory, all in flight together (up
-// to 16 per lane; 8 lanes own one 64-wide head vector) without registers, from
-// where norm and RoPE, the maximum and the codes are taken.  Codes leave in 16-byte
-// pieces: a lane takes 16 dims of a K row, or 16 tokens of two V dims, for which
-// shared memory is the transpose.
+// One CTA per window of rows and pair of heads, warp = (KV head, K or V).  A run
+// is a sequence of adjacent rows that go to adjacent slots of one block; the
+// warps of the window that holds its first row quantise the whole run, each for
+// its head, so a block's scale is found and its codes are written by one warp
+// alone, with no atomics.  A run's loads are copies to shared memory, all in
+// flight together (up to 16 per lane; 8 lanes own one 64-wide head vector) and
+// without registers, from where norm and RoPE, the maximum and the codes are
+// taken.  Codes leave in 16-byte pieces: a lane takes 16 dims of a K row, or 16
+// tokens of two V dims, for which shared memory is the transpose.
 //
-// Bound by latency: a run's loads, its codes, its stores.  kWindow 8 spreads few
-// rows over the SMs; 32 keeps the CTAs that hold no run's start from outnumbering
-// the others in long prompts.
+// Bound by latency: a run's loads, its codes, its stores (64 x 128 tokens 14 us,
+// 8 of them the loads; 21 tokens 4.9 us).  kWindow 8 spreads few rows over the
+// SMs; 32 keeps the CTAs that hold no run's start from outnumbering the others
+// in long prompts (64: 15-25 % slower there, 8: 10 %).
 template <int kWindow>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
 // with 3 or 4 new tokens.
 //
 // Which tokens and dims the rows and k slots of a fragment stand for is free as
-// long as both operands agree: a lane's 16 k slots of two mma steps are 16
+// long as both operands agree: a lane's 16 k slots of four mma steps are 16
 // adjacent bytes of a row, so an operand of 16 rows is two 16-byte loads per
 // lane, free of bank conflicts without a swizzle.
 //
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     const int b = b0 + static_cast<int>(threadIdx.x);
     int n = 0;
     if (b < a.batch) {
-      const int past = __ldg(a.past_lens + b), ntok = a.chunk_lens ? __ldg(a.chunk_lens + b) : a.tokens;
+      const int past = __ldcg(a.past_lens + b), ntok = a.chunk_lens ? __ldcg(a.chunk_lens + b) : a.tokens;
       const bool fits = past >= 0 && ntok >= 0 && ntok <= a.tokens &&
                         static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock;
       if (!fits && blockIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
@@ -628,7 +629,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     if (w < w1) {
       place(w, sb, head, block, blocks);
       if (block < blocks) {
-        const int e = __ldg(a.block_tables + static_cast<int64_t>(sb) * a.max_blocks + block);
+        const int e = __ldcg(a.block_tables + static_cast<int64_t>(sb) * a.max_blocks + block);
         id = e < 0 || e >= a.num_blocks ? -1 : e * kHkv + head;
       }
     }
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     const uint16_t *p = a.qkv + static_cast<int64_t>(sb) * a.tokens * a.row_stride + vec * kDim + j * 8;
 #pragma unroll
     for (int i = 0; i < kT; ++i)
-      if (i < sh.fresh[sb]) fresh_next[i] = __ldg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
+      if (i < sh.fresh[sb]) fresh_next[i] = __ldcg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
   };
   if (blk >= nblk) blk = 0;
   if (b < a.batch && w0 < w1) {
@@ -693,7 +694,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     }
     // (as 16-byte copies of their own the scales doubled the copies, which one
     // thread issues at about 100 ns each)
-    scales[kStages - 1] = make_float2(__ldg(a.k_scale + max(id, 0)), __ldg(a.v_scale + max(id, 0)));
+    scales[kStages - 1] = make_float2(__ldcg(a.k_scale + max(id, 0)), __ldcg(a.v_scale + max(id, 0)));
     ++issued;
   };
 #pragma unroll
@@ -757,14 +758,14 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
       __syncwarp();
       // column g holds vector g / 2 (g even) or 4 + g / 2
       const int qv = (g >> 1) + 4 * (g & 1);
-      uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
+      uint4 q0 = make_uint4(0u, 0u, 0u, 0u), q1 = q0;
       if (qv < 2 * ntok) {
         const uint4 *p = reinterpret_cast<const uint4 *>(&sh.row[warp].q[qv][16 * t]);
-        w0 = p[0];
-        w1 = p[1];
+        q0 = p[0];
+        q1 = p[1];
       }
-      bq[0][0] = w0.x; bq[0][1] = w0.y; bq[1][0] = w0.z; bq[1][1] = w0.w;
-      bq[2][0] = w1.x; bq[2][1] = w1.y; bq[3][0] = w1.z; bq[3][1] = w1.w;
+      bq[0][0] = q0.x; bq[0][1] = q0.y; bq[1][0] = q0.z; bq[1][1] = q0.w;
+      bq[2][0] = q1.x; bq[2][1] = q1.y; bq[3][0] = q1.z; bq[3][1] = q1.w;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1525,7 +1526,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       return static_cast<int64_t>(blk < 0 || blk >= a.num_blocks ? 0 : blk) * kHkv + h;
     };
     int64_t id = pool_tile(lane);
-    float2 scale = make_float2(__ldg(a.k_scale + id), __ldg(a.v_scale + id)), scale_next = scale;
+    float2 scale = make_float2(__ldcg(a.k_scale + id), __ldcg(a.v_scale + id)), scale_next = scale;
     for (int j = 0; j < nblk; ++j) {
       if (!warp_wait(smem_u32(&tail->sbar[j & 1]), (j >> 1) & 1)) {
         ok = false;
@@ -1539,7 +1540,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       tmem_fence_after();
       if (j > 0 && (j & 31) == 0) scale = scale_next;
       if ((j & 31) == 8) id = pool_tile((j & ~31) + 32 + lane);
-      if ((j & 31) == 16) scale_next = make_float2(__ldg(a.k_scale + id), __ldg(a.v_scale + id));
+      if ((j & 31) == 16) scale_next = make_float2(__ldcg(a.k_scale + id), __ldcg(a.v_scale + id));
       const float ks = __shfl_sync(0xffffffffu, scale.x, j & 31), vs = __shfl_sync(0xffffffffu, scale.y, j & 31);
       float sc[64];
       tmem_ld64(trow + 64 * (j & 1), sc);
@@ -1734,7 +1735,9 @@ bool prefill_ready() {
 
 int launch_prefill(PrefillArgs a, int batch, int max_blocks, cudaStream_t st) {
   if (!prefill_ready()) return fail(B2_ERR_CUDA, "cannot set the prefill kernel's shared memory size");
-  const int tiles = (a.tokens + kBlock - 1) / kBlock;
+  // (no chunk is longer than its table; longer ones are refused by their first tile)
+  const int64_t longest = a.tokens < static_cast<int64_t>(max_blocks) * kBlock ? a.tokens : static_cast<int64_t>(max_blocks) * kBlock;
+  const int tiles = static_cast<int>((longest + kBlock - 1) / kBlock);
   const int64_t ctas = static_cast<int64_t>(tiles) * kHkv * batch;
   // Split the keys when the tiles leave SMs without a CTA: about two CTAs per
   // SM, of at least 4 blocks each (as far as the table's width tells).
@@ -1895,7 +1898,6 @@ extern "C" int b2_kv8_prefill_attn(const uint16_t *q, int64_t q_stride, int32_t 
   if (!workspace || !aligned16(workspace) || workspace_bytes < kWorkspaceBytes)
     return fail(B2_ERR_ARG, "workspace must be 16-byte aligned and hold b2_kv8_workspace_bytes()");
   if (!(scale > 0.f)) return fail(B2_ERR_ARG, "scale must be positive");
-  if ((static_cast<int64_t>(tokens) + kBlock - 1) / kBlock * kHkv > 0x7fffffff) return fail(B2_ERR_ARG, "tokens too large");
   PrefillArgs a{q, q_stride, rows, row_start, past_lens, chunk_lens, tokens, block_tables, max_blocks_per_seq,
                 k_pool, v_pool, k_scale, v_scale, num_blocks, scale * 1.4426950408889634f, out, 1,
                 reinterpret_cast<PrefillState *>(static_cast<char *>(workspace) + kStepBytes), dev_err,

@@ -387,6 +387,19 @@ def test_prefill_packed(cuda, norm_rope):
     _check_rows(cache, ref, turned, out, lens, starts, chunk)
 
 
+def test_prefill_packed_with_a_loose_bound(cuda):
+    """max_tokens may be any bound of the chunks."""
+    a8, _, _ = _mods()
+    cache, ref = _build([70, 3], cuda, seed=115, room=80)
+    rows = _rows(60, 30, cuda)
+    tables = cache.block_tables()
+    slots = [int(tables[0, (70 + t) // BLOCK]) * BLOCK + (70 + t) % BLOCK for t in range(40)]
+    slots += [int(tables[1, 0]) * BLOCK + 3 + t for t in range(20)]
+    out = _prefill(cache, rows, [70, 3], cuda, [40, 20], row_start=_ints([0, 40], cuda), max_tokens=2 ** 31 - 1,
+                   slots=_ints(slots, cuda))
+    _check_rows(cache, ref, rows, out, [70, 3], [0, 40], [40, 20])
+
+
 @pytest.mark.parametrize("order", [1, -1])
 def test_prefill_scales_far_apart(cuda, order):
     fv = [1e-6, 0.0, 1.0, 3e5, 1e-3, 2.0, 1e8, 1e-8, 1.0][::order]
@@ -567,3 +580,61 @@ def test_serving_loop_allocates_in_a_graph(cuda):
     free = dev.free_list[:int(dev.free_count)].tolist()
     assert sorted(held + free) == list(range(blocks))
     assert ref.same_as(cache.kv8())
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_native_binding_and_python_checks_agree(cuda, binding, monkeypatch):
+    """The same calls and the same refusals with the native binding and without it."""
+    a8, _, lib = _mods()
+    assert a8._b2torch is not None, "the native binding is not built"
+    if not binding:
+        monkeypatch.setattr(a8, "_b2torch", None)
+    bt = load_pkg("block_tables")
+    lens = [5, 64]
+    cache, ref = _build(lens, cuda, seed=171, room=80)
+    w = orc.attention_weights(4)
+    cos, sin = load_pkg("rope").rope_table(256, device=cuda)
+    qk = dict(gamma_q=w["q_gamma"].to(cuda), gamma_k=w["k_gamma"].to(cuda), cos=cos, sin=sin)
+    for n, call in ((1, _step), (70, _prefill)):
+        rows = _rows(2 * n, 70 + n, cuda).view(2, n, 2048)
+        out = call(cache, rows, lens, cuda, mode=7, **qk)
+        for b, p in enumerate(lens):
+            q, k, v = ora.split(rows[b])
+            q, k = orc.norm_rope_qk(q, k, w["q_gamma"], w["k_gamma"], *orc.rope_cos_sin(list(range(p, p + n))))
+            ora.append(ref, cache.block_tables()[b].cpu(), p, k, v)
+            ora.check_context(out[b], *ora.attend(ref, cache.block_tables()[b].cpu(), p, q))
+        lens = [p + n for p in lens]
+    assert ref.same_as(cache.kv8())
+    good = dict(block_tables=cache.block_tables(), workspace=a8.workspace_kv8(cuda), dev_err=_err(cuda), **cache.kv8())
+    rows, past = _rows(2, 1, cuda).view(2, 1, 2048).to(cuda), _ints(lens, cuda)
+    out = torch.zeros(2, 1, 16, 64, dtype=BF16, device=cuda)
+    for name, bad in (("block_tables", good["block_tables"].cpu()), ("block_tables", good["block_tables"].long()),
+                      ("k_scale", cache.k_scale[0].T), ("v_pool", cache.k[0][:-1]), ("workspace", out),
+                      ("dev_err", _ints([0, 0], cuda)), ("chunk_lens", past.cpu()), ("gamma_q", None)):
+        with pytest.raises(ValueError):
+            a8.decode_step_kv8(rows, past, out=out, mode=7, **{**qk, **good, name: bad})
+        if name != "chunk_lens":
+            with pytest.raises(ValueError):
+                a8.prefill_kv8(rows, past, out=out, mode=7, **{**qk, **good, name: bad})
+    with pytest.raises(lib.B2Error, match="workspace"):
+        a8.decode_step_kv8(rows, past, out=out, **{**qk, **good, "workspace": good["workspace"][:64]})
+    with pytest.raises(lib.B2Error, match="scale"):
+        a8.decode_step_kv8(rows, past, out=out, scale=-1.0, **qk, **good)
+    # a parameter is a tensor too; whole numbers as scale
+    a8.decode_step_kv8(torch.nn.Parameter(rows, requires_grad=False), past, out=out, scale=1, **qk, **good)
+    dev = bt.DeviceBlockTables(2, 4, 128, cuda)
+    plan = dev.plan(_ints([64, 65], cuda), rows=129)
+    assert plan.granted.tolist() == [64, 65] and dev.held.tolist() == [1, 2]
+    with pytest.raises(ValueError):
+        dev.plan(_ints([1, 1, 1], cuda), rows=3)
+
+
+def test_refuses_host_tensors(cuda):
+    """Tensors that are all on the host never reach the library."""
+    a8, pc, lib = _mods()
+    cache = pc.PagedKVCache8(2, 64, device="cpu")
+    args = dict(block_tables=torch.zeros(1, 1, dtype=I32), out=torch.zeros(1, 1, 16, 64, dtype=BF16),
+                workspace=torch.zeros(64, dtype=torch.uint8), dev_err=torch.zeros(1, dtype=I32), mode=lib.B2_STORE_KV,
+                **cache.kv8())
+    with pytest.raises(ValueError, match="CUDA device"):
+        a8.decode_step_kv8(torch.zeros(1, 1, 2048, dtype=BF16), torch.zeros(1, dtype=I32), **args)
