@@ -67,16 +67,19 @@ int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t rows,
  * attention of token t over past_lens[b] + t + 1 tokens.  Without B2_STORE_KV
  * the new tokens' k/v are in the cache already.
  *
- * qkv        row b * tokens + t; chunk_lens[b] (0 .. tokens; NULL: tokens) of
- *            them are there.  A sequence with none is skipped.
- * out        bf16 [batch][tokens][16][64]; rows past a sequence's chunk are
- *            left as they were.
+ * qkv        rows of row_stride, `rows` of them; token t of sequence b is row
+ *            row_start[b] + t (NULL: b * tokens + t).  chunk_lens[b] (0 ..
+ *            tokens; NULL: tokens) tokens are there; a sequence with none is
+ *            skipped, one that would leave the rows is refused
+ *            (B2_DEV_BAD_LENGTH).
+ * out        bf16 [rows][16][64]; rows of no token are left as they were.
  * workspace  b2_kv8_workspace_bytes() bytes, 16-byte aligned, zeroed once; a
  *            call that completes leaves it ready for the next.  Calls that
  *            share a workspace must not overlap on the GPU.  After a device
  *            error, zero it again.
  */
-int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t tokens, const int32_t *chunk_lens,
+int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t rows, const int32_t *row_start,
+                       int32_t tokens, const int32_t *chunk_lens,
                        const uint16_t *gamma_q, const uint16_t *gamma_k, float eps,
                        const uint16_t *rope_cos, const uint16_t *rope_sin, int32_t rope_rows,
                        const int32_t *past_lens, const int32_t *block_tables, int32_t max_blocks_per_seq,

@@ -191,7 +191,8 @@ SIGNATURES = {
         _p, _i32, _p, _p,    # q_out, mode, dev_err, stream
     ]),
     "b2_kv8_decode_step": (ctypes.c_int, [
-        _p, _i64, _i32, _p,  # qkv, row_stride, tokens, chunk_lens
+        _p, _i64, _i32, _p,  # qkv, row_stride, rows, row_start
+        _i32, _p,            # tokens, chunk_lens
         _p, _p, _f32,        # gamma_q, gamma_k, eps
         _p, _p, _i32,        # rope_cos, rope_sin, rope_rows
         _p, _p, _i32,        # past_lens, block_tables, max_blocks_per_seq

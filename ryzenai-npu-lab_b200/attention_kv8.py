@@ -178,34 +178,47 @@ def decode_step_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch
                     workspace: torch.Tensor, dev_err: torch.Tensor, chunk_lens: torch.Tensor | None = None,
                     gamma_q: torch.Tensor | None = None, gamma_k: torch.Tensor | None = None,
                     cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, mode: int = NORM_ROPE_STORE,
-                    eps: float = EPS, scale: float = SCALE, stream: torch.cuda.Stream | None = None) -> None:
-    """One decode step over the 8-bit cache (b2_kv8_decode_step): qkv bf16
-    [B, T, >= 2048] raw projections of T = 1 to 4 new tokens per sequence at
-    positions past_lens[b] + t, chunk_lens[b] (0 to T; None: T) of them there.
-    Appends their k/v and writes the contexts into out [B, T, 16, 64]; rows
-    past a sequence's chunk stay as they were.  `mode` as decode_step's."""
+                    eps: float = EPS, scale: float = SCALE, stream: torch.cuda.Stream | None = None,
+                    row_start: torch.Tensor | None = None, max_tokens: int | None = None) -> None:
+    """One decode step over the 8-bit cache (b2_kv8_decode_step): raw
+    projections of up to 4 new tokens per sequence at positions past_lens[b] + t.
+
+    Padded: qkv bf16 [B, T, >= 2048], T of 1 to 4, chunk_lens[b] (0 to T; None:
+    T) of them there.
+    Packed: qkv bf16 [rows, >= 2048], sequence b's chunk_lens[b] <= max_tokens
+    tokens (None: max_tokens) from row row_start[b] on.
+
+    Appends their k/v and writes the contexts into out ([B, T, 16, 64], packed
+    [rows, 16, 64]); rows of no token stay as they were.  The sequences' last
+    blocks are distinct: no two entries append to one sequence.  `mode` as
+    decode_step's."""
     native, raw = _native(qkv, stream)
     if native is not None:
         rc = native.step(qkv, past_lens, k_pool, v_pool, k_scale, v_scale, block_tables, out, workspace, dev_err,
-                         chunk_lens, gamma_q, gamma_k, cos, sin, mode, eps, scale, raw)
+                         chunk_lens, gamma_q, gamma_k, cos, sin, mode, eps, scale, raw, row_start, max_tokens)
         if rc == 0:
             return
         if rc is not None:
             _lib.check(rc, "b2_kv8_decode_step")
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 3 or qkv.shape[2] < QKV_WIDTH:
-        raise ValueError(f"qkv must be [batch, tokens, >= {QKV_WIDTH}]")
-    b, t, width = qkv.shape
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3) or qkv.shape[-1] < QKV_WIDTH:
+        raise ValueError(f"qkv must be [rows, >= {QKV_WIDTH}] or [batch, tokens, >= {QKV_WIDTH}]")
+    padded, width = qkv.dim() == 3, qkv.shape[-1]
+    if padded != (row_start is None) or padded != (max_tokens is None):
+        raise ValueError("packed qkv [rows, width] needs row_start and max_tokens, padded qkv neither")
+    t = qkv.shape[1] if padded else int(max_tokens)
     if not 1 <= t <= MAX_STEP_TOKENS:
         raise ValueError(f"tokens must be in [1, {MAX_STEP_TOKENS}], got {t}")
     index = qkv.get_device()
-    q = _is(qkv, "qkv", _BF16, qkv, index, (b, t, width))
-    tb, table_width, tables, past, chunk = _need_tables(block_tables, past_lens, chunk_lens, qkv, index)
-    if tb != b:
-        raise ValueError(f"block_tables must have {b} rows, got {tb}")
-    _launch("b2_kv8_decode_step", index, stream, q, width, t, chunk,
+    q = _is(qkv, "qkv", _BF16, qkv, index, qkv.shape)
+    b, table_width, tables, past, chunk = _need_tables(block_tables, past_lens, chunk_lens, qkv, index)
+    if padded and b != qkv.shape[0]:
+        raise ValueError(f"block_tables must have {qkv.shape[0]} rows, got {b}")
+    rows = b * t if padded else qkv.shape[0]
+    start = None if padded else _is(row_start, "row_start", _I32, qkv, index, (b,))
+    _launch("b2_kv8_decode_step", index, stream, q, width, rows, start, t, chunk,
             *_need_qk(mode, gamma_q, gamma_k, eps, cos, sin, qkv, index), past, tables, table_width,
             *_need_cache(k_pool, v_pool, k_scale, v_scale, qkv, index), b, scale, mode,
-            _is(out, "out", _BF16, qkv, index, (b, t, HQ, D)), *_need_workspace(workspace, qkv, index),
+            _is(out, "out", _BF16, qkv, index, (*qkv.shape[:-1], HQ, D)), *_need_workspace(workspace, qkv, index),
             _need_err(dev_err, qkv, index))
 
 
@@ -306,10 +319,20 @@ class PagedDecodeAttentionKV8:
                 "gamma_k": self.gamma_k, "cos": self.cos, "sin": self.sin, "eps": self.eps, "scale": self.scale}
 
     def step(self, layer: int, qkv: torch.Tensor, past_lens: torch.Tensor, block_tables: torch.Tensor, *,
-             chunk_lens: torch.Tensor | None = None, out: torch.Tensor | None = None,
+             chunk_lens: torch.Tensor | None = None, row_start: torch.Tensor | None = None,
+             max_tokens: int | None = None, out: torch.Tensor | None = None,
              stream: torch.cuda.Stream | None = None) -> torch.Tensor:
-        """qkv bf16 [B, W] (one token per sequence) or [B, T, W] raw projections;
-        returns the contexts [B, 16, 64] or [B, T, 16, 64]."""
+        """qkv bf16 [B, W] (one token per sequence), [B, T, W] or, with row_start
+        and max_tokens, packed [rows, W] raw projections; returns the contexts
+        [B, 16, 64], [B, T, 16, 64] or [rows, 16, 64]."""
+        if row_start is not None:
+            if out is None:
+                if qkv.shape[0] > self.out.shape[0]:
+                    raise ValueError(f"{qkv.shape[0]} rows > max_batch x max_tokens {self.out.shape[0]}")
+                out = self.out[:qkv.shape[0]]
+            decode_step_kv8(qkv, past_lens, block_tables=block_tables, chunk_lens=chunk_lens, row_start=row_start,
+                            max_tokens=max_tokens, out=out, stream=stream, **self._common(layer))
+            return out
         rows = qkv if qkv.dim() == 3 else qkv.unsqueeze(1)
         b, t = rows.shape[:2]
         if out is None:

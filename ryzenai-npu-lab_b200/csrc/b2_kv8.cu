@@ -433,6 +433,8 @@ static_assert(2 * step_warps<2>() <= 32 && 2 * step_warps<kMaxStepTokens>() <= 3
 struct StepArgs {
   const uint16_t *qkv;
   int64_t row_stride;
+  int rows;
+  const int32_t *row_start;
   int tokens;
   const int32_t *chunk_lens;
   const uint16_t *gamma_q, *gamma_k;
@@ -564,6 +566,10 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  // the row of a sequence's first new token
+  auto row_of = [&](int sb) -> int64_t {
+    return a.row_start ? __ldcg(a.row_start + sb) : static_cast<int64_t>(sb) * a.tokens;
+  };
   // The batch's work as a line: sequence b has the positions [pos[b], pos[b + 1]),
   // its 8 heads' segments in turn, a segment its tiles and kSegmentCost more
   // positions that stand for the cost of its start and end.
@@ -573,8 +579,10 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     int n = 0;
     if (b < a.batch) {
       const int past = __ldcg(a.past_lens + b), ntok = a.chunk_lens ? __ldcg(a.chunk_lens + b) : a.tokens;
+      const int64_t first = row_of(b);
       const bool fits = past >= 0 && ntok >= 0 && ntok <= a.tokens &&
-                        static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock;
+                        static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock &&
+                        first >= 0 && first + ntok <= a.rows;
       if (!fits && blockIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
       if (fits && ntok > 0) n = ((past + ntok + kBlock - 1) / kBlock + kSegmentCost) * kHkv;
       sh.past[b] = past;
@@ -660,7 +668,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
   uint4 fresh[kT], fresh_next[kT];
   auto fetch = [&](int sb, int head) {
     const int vec = grp < 2 ? 2 * head + grp : (grp == 2 ? kHq + head : kHq + kHkv + head);
-    const uint16_t *p = a.qkv + static_cast<int64_t>(sb) * a.tokens * a.row_stride + vec * kDim + j * 8;
+    const uint16_t *p = a.qkv + row_of(sb) * a.row_stride + vec * kDim + j * 8;
 #pragma unroll
     for (int i = 0; i < kT; ++i)
       if (i < sh.fresh[sb]) fresh_next[i] = __ldcg(reinterpret_cast<const uint4 *>(p + i * a.row_stride));
@@ -999,7 +1007,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
         __syncwarp();
         for (int c8 = lane; c8 < 2 * ntok * 8; c8 += 32) {
           const int v = c8 >> 3;
-          *reinterpret_cast<uint4 *>(a.out + ((static_cast<int64_t>(b) * a.tokens + (v >> 1)) * kHq + 2 * h + (v & 1)) * kDim +
+          *reinterpret_cast<uint4 *>(a.out + ((row_of(b) + (v >> 1)) * kHq + 2 * h + (v & 1)) * kDim +
                                      8 * (c8 & 7)) = *reinterpret_cast<const uint4 *>(&sh.row[warp].out[v][8 * (c8 & 7)]);
         }
         __syncwarp();
@@ -1078,7 +1086,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
           sum.add(i, *reinterpret_cast<const float4 *>(&state(e0 + i)->o[vec][d]), lane);
         }
       }
-      uint16_t *dst = a.out + ((static_cast<int64_t>(sb) * a.tokens + v) * kHq + 2 * hh) * kDim;
+      uint16_t *dst = a.out + ((row_of(sb) + v) * kHq + 2 * hh) * kDim;
       if (cf == cl) {
         sum.write(dst, lane);
         continue;
@@ -1176,9 +1184,14 @@ int launch_step(StepArgs a, cudaStream_t st) {
     cfg.numAttrs = 1;
     const int rc = launched(cudaLaunchKernelEx(&cfg, kv8_step_kernel<kT>, a), "kv8_step_kernel");
     if (rc) return rc;
-    const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens;
-    a.qkv += rows * a.row_stride;
-    a.out += rows * kHq * kDim;
+    if (a.row_start) {
+      a.row_start += a.batch;
+    } else {
+      const int64_t rows = static_cast<int64_t>(a.batch) * a.tokens;
+      a.qkv += rows * a.row_stride;
+      a.out += rows * kHq * kDim;
+      a.rows -= static_cast<int>(rows);
+    }
     a.past_lens += a.batch;
     if (a.chunk_lens) a.chunk_lens += a.batch;
     a.block_tables += static_cast<int64_t>(a.batch) * a.max_blocks;
@@ -1851,17 +1864,19 @@ extern "C" int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t ro
   return rows <= 1024 ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
 }
 
-extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t tokens, const int32_t *chunk_lens,
+extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t rows, const int32_t *row_start,
+                                  int32_t tokens, const int32_t *chunk_lens,
                                   const uint16_t *gamma_q, const uint16_t *gamma_k, float eps,
                                   const uint16_t *rope_cos, const uint16_t *rope_sin, int32_t rope_rows,
                                   const int32_t *past_lens, const int32_t *block_tables, int32_t max_blocks_per_seq,
                                   uint8_t *k_pool, uint8_t *v_pool, float *k_scale, float *v_scale,
                                   int32_t num_blocks, int32_t batch, float scale, int32_t mode, uint16_t *out,
                                   void *workspace, int64_t workspace_bytes, int32_t *dev_err, void *stream) {
-  if (batch < 0) return fail(B2_ERR_ARG, "batch must be >= 0");
+  if (batch < 0 || rows < 0) return fail(B2_ERR_ARG, "batch and rows must be >= 0");
   if (tokens < 1 || tokens > kMaxStepTokens) return fail(B2_ERR_ARG, "tokens must be in [1, 4]");
   if (batch == 0) return b2_clear_error();
-  if (static_cast<int64_t>(batch) * tokens > 0x7fffffff) return fail(B2_ERR_ARG, "batch * tokens too large");
+  if (!row_start && static_cast<int64_t>(batch) * tokens > rows)
+    return fail(B2_ERR_ARG, "without row_start, rows must be >= batch * tokens");
   int rc = check_rows(qkv, row_stride, mode, gamma_q, gamma_k, rope_cos, rope_sin, rope_rows);
   if (!rc) rc = check_tables(block_tables, max_blocks_per_seq, past_lens);
   if (!rc) rc = check_cache(k_pool, v_pool, k_scale, v_scale, num_blocks);
@@ -1870,8 +1885,8 @@ extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32
   if (!workspace || !aligned16(workspace) || workspace_bytes < kWorkspaceBytes)
     return fail(B2_ERR_ARG, "workspace must be 16-byte aligned and hold b2_kv8_workspace_bytes()");
   if (!(scale > 0.f)) return fail(B2_ERR_ARG, "scale must be positive");
-  StepArgs a{qkv, row_stride, tokens, chunk_lens, gamma_q, gamma_k, eps, rope_cos, rope_sin, rope_rows, past_lens,
-             block_tables, max_blocks_per_seq, k_pool, v_pool, k_scale, v_scale, num_blocks, batch,
+  StepArgs a{qkv, row_stride, rows, row_start, tokens, chunk_lens, gamma_q, gamma_k, eps, rope_cos, rope_sin, rope_rows,
+             past_lens, block_tables, max_blocks_per_seq, k_pool, v_pool, k_scale, v_scale, num_blocks, batch,
              scale * 1.4426950408889634f, mode, out, static_cast<int32_t *>(workspace),
              reinterpret_cast<float *>(static_cast<char *>(workspace) + kCounterBytes), dev_err, b2_wait_limit_ns()};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

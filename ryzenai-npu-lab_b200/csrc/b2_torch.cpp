@@ -21,9 +21,9 @@ namespace {
 constexpr int64_t kHq = 16, kHkv = 8, kDim = 64, kBlock = 64, kWidth = 2048;
 constexpr int kNorm = 1, kRope = 2, kStore = 4;
 
-using StepFn = int (*)(const void *, int64_t, int32_t, const void *, const void *, const void *, float, const void *,
-                       const void *, int32_t, const void *, const void *, int32_t, void *, void *, void *, void *,
-                       int32_t, int32_t, float, int32_t, void *, void *, int64_t, void *, void *);
+using StepFn = int (*)(const void *, int64_t, int32_t, const void *, int32_t, const void *, const void *, const void *,
+                       float, const void *, const void *, int32_t, const void *, const void *, int32_t, void *, void *,
+                       void *, void *, int32_t, int32_t, float, int32_t, void *, void *, int64_t, void *, void *);
 using AppendFn = int (*)(const void *, int64_t, int32_t, const void *, const void *, const void *, const void *, int32_t,
                          const void *, int32_t, const void *, const void *, float, const void *, const void *, int32_t,
                          void *, void *, void *, void *, int32_t, void *, int32_t, void *, void *);
@@ -141,31 +141,37 @@ bool small(std::initializer_list<int64_t> values) {
 PyObject *not_here() { Py_RETURN_NONE; }
 
 // qkv, past_lens, k, v, k_scale, v_scale, block_tables, out, workspace, dev_err, chunk_lens, gamma_q, gamma_k, cos,
-// sin, mode, eps, scale, stream
+// sin, mode, eps, scale, stream, row_start, max_tokens
 PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  if (n != 19 || !g_step) return not_here();
+  if (n != 21 || !g_step) return not_here();
   Args a(args);
   const at::Tensor *qkv = a.tensor(args[0]);
-  if (!qkv || qkv->dim() != 3 || !qkv->is_cuda()) return not_here();
+  if (!qkv || (qkv->dim() != 2 && qkv->dim() != 3) || !qkv->is_cuda()) return not_here();
   a.index = qkv->get_device();
-  const int64_t b = qkv->size(0), t = qkv->size(1), width = qkv->size(2);
+  const bool padded = qkv->dim() == 3;
   const at::Tensor *tables = a.plain(6, kI32);
-  if (t < 1 || t > 4 || width < kWidth || !tables || tables->dim() != 2) return not_here();
-  const int64_t cols = tables->size(1), mode = a.whole(15);
-  void *q = a.ptr(0, kBf16, {b, t, width}), *past = a.ptr(1, kI32, {b}), *table = a.ptr(6, kI32, {b, cols});
+  if (!tables || tables->dim() != 2 || !a.plain(0, kBf16) || (args[19] == Py_None) != padded ||
+      (args[20] == Py_None) != padded)
+    return not_here();
+  const int64_t b = tables->size(0), cols = tables->size(1), mode = a.whole(15);
+  const int64_t t = padded ? qkv->size(1) : a.whole(20), width = qkv->size(-1);
+  const int64_t rows = padded ? b * t : qkv->size(0);
+  if (t < 1 || t > 4 || width < kWidth || (padded && qkv->size(0) != b)) return not_here();
+  void *q = qkv->data_ptr(), *past = a.ptr(1, kI32, {b}), *table = a.ptr(6, kI32, {b, cols});
+  void *start = a.ptr_or_null(19, kI32, {b});
   const Cache c = cache_args(a, 2);
-  void *out = a.ptr(7, kBf16, {b, t, kHq, kDim});
+  void *out = padded ? a.ptr(7, kBf16, {b, t, kHq, kDim}) : a.ptr(7, kBf16, {rows, kHq, kDim});
   const at::Tensor *work = a.plain(8, at::kByte);
   void *err = a.ptr(9, kI32, {1}), *chunk = a.ptr_or_null(10, kI32, {b});
   const QkArgs qk = qk_args(a, 11, mode);
   const float eps = a.number(16), scale = a.number(17);
   const int64_t stream = PyLong_AsLongLong(args[18]);
-  if (!a.ok || !small({b, width, cols, c.blocks, qk.rows})) return not_here();
-  return PyLong_FromLong(g_step(q, width, static_cast<int32_t>(t), chunk, qk.gq, qk.gk, eps, qk.cos, qk.sin,
-                                static_cast<int32_t>(qk.rows), past, table, static_cast<int32_t>(cols), c.k, c.v, c.ks,
-                                c.vs, static_cast<int32_t>(c.blocks), static_cast<int32_t>(b), scale,
-                                static_cast<int32_t>(mode), out, work->data_ptr(), work->numel(), err,
-                                reinterpret_cast<void *>(stream)));
+  if (!a.ok || !small({b, rows, width, cols, c.blocks, qk.rows})) return not_here();
+  return PyLong_FromLong(g_step(q, width, static_cast<int32_t>(rows), start, static_cast<int32_t>(t), chunk, qk.gq,
+                                qk.gk, eps, qk.cos, qk.sin, static_cast<int32_t>(qk.rows), past, table,
+                                static_cast<int32_t>(cols), c.k, c.v, c.ks, c.vs, static_cast<int32_t>(c.blocks),
+                                static_cast<int32_t>(b), scale, static_cast<int32_t>(mode), out, work->data_ptr(),
+                                work->numel(), err, reinterpret_cast<void *>(stream)));
 }
 
 // qkv, past_lens, k, v, k_scale, v_scale, block_tables, out, workspace, dev_err, chunk_lens, gamma_q, gamma_k, cos,

@@ -119,12 +119,14 @@ def test_abi_argument_errors_without_gpu():
         assert text in lib.last_error(), lib.last_error()
 
     def step(qkv=buf, stride=2048, tokens=1, width=4, k=buf, ks=buf, blocks=8, batch=1, scale=0.125, mode=4, out=buf,
-             ws=buf, size=nbytes, gamma=None, rope=None):
-        return c.b2_kv8_decode_step(qkv, stride, tokens, None, gamma, gamma, f(1e-5), rope, rope, 0, buf, buf, width, k,
+             ws=buf, size=nbytes, gamma=None, rope=None, rows=64, start=None):
+        return c.b2_kv8_decode_step(qkv, stride, rows, start, tokens, None, gamma, gamma, f(1e-5), rope, rope, 0, buf, buf, width, k,
                                     buf, ks, buf, blocks, batch, f(scale), mode, out, ws, size, buf, None)
     refused(step(tokens=5), "tokens")
     refused(step(tokens=0), "tokens")
     refused(step(batch=-1), "batch")
+    refused(step(rows=-1, start=buf), "rows")
+    refused(step(batch=17, tokens=4, rows=67), "row_start")
     refused(step(stride=2044), "row_stride")
     refused(step(qkv=buf + 8), "qkv")
     refused(step(width=1 << 25), "max_blocks_per_seq")

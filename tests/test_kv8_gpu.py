@@ -387,6 +387,66 @@ def test_prefill_packed(cuda, norm_rope):
     _check_rows(cache, ref, turned, out, lens, starts, chunk)
 
 
+@pytest.mark.parametrize("top", [1, 2, 4])
+@pytest.mark.parametrize("norm_rope", [False, True])
+@pytest.mark.parametrize("binding", [True, False])
+def test_step_packed(cuda, top, norm_rope, binding, monkeypatch):
+    """Packed rows with gaps and empty chunks; a sequence behind the last row is refused, the others are not."""
+    a8, _, lib = _mods()
+    if not binding:
+        monkeypatch.setattr(a8, "_b2torch", None)
+    lens, chunk, starts = [5, 0, 130, 64, 63], [top, 1, top, 0, 1], [1, 1 + top, 4 + top, 4 + 2 * top, 4 + 2 * top]
+    n = 6 + 2 * top
+    cache, ref = _build(lens, cuda, seed=113, room=20)
+    rows = _rows(n, 31, cuda)
+    kw = dict(row_start=_ints(starts, cuda), max_tokens=top)
+    turned = rows.clone()
+    if norm_rope:
+        w = orc.attention_weights(5)
+        cos, sin = load_pkg("rope").rope_table(256, device=cuda)
+        kw |= dict(mode=7, gamma_q=w["q_gamma"].to(cuda), gamma_k=w["k_gamma"].to(cuda), cos=cos, sin=sin)
+        for p, r, m in zip(lens, starts, chunk):
+            if m:
+                q, k, v = ora.split(rows[r:r + m])
+                q, k = orc.norm_rope_qk(q, k, w["q_gamma"], w["k_gamma"], *orc.rope_cos_sin(list(range(p, p + m))))
+                turned[r:r + m] = torch.cat([q.reshape(m, -1), k.reshape(m, -1), v.reshape(m, -1)], 1)
+    out = torch.zeros(n, 16, 64, dtype=BF16, device=cuda)
+    kept = [t.clone() for t in cache.kv8().values()]
+    for last, flagged in ((n, True), (starts[4], False)):
+        # the refused call first: it leaves its own sequence and only that one out
+        for t, was in zip(cache.kv8().values(), kept):
+            t.copy_(was)
+        out.zero_()
+        kw["row_start"] = _ints(starts[:4] + [last], cuda)
+        err = _err(cuda)
+        a8.decode_step_kv8(rows.to(cuda), _ints(lens, cuda), block_tables=cache.block_tables(), out=out,
+                           workspace=a8.workspace_kv8(cuda), dev_err=err, chunk_lens=_ints(chunk, cuda),
+                           **{"mode": lib.B2_STORE_KV, **kw}, **cache.kv8())
+        assert err.item() == (lib.B2_DEV_BAD_LENGTH if flagged else 0)
+        if flagged:
+            assert not bool(out[starts[4]:].any())
+    _check_rows(cache, ref, turned, out, lens, starts, chunk)
+    call = dict(block_tables=cache.block_tables(), out=out, workspace=a8.workspace_kv8(cuda), dev_err=_err(cuda),
+                **{"mode": lib.B2_STORE_KV, **kw}, **cache.kv8())
+    for bad in (dict(row_start=None), dict(max_tokens=None), dict(max_tokens=0), dict(max_tokens=5),
+                dict(row_start=_ints(starts[:4], cuda)), dict(row_start=_ints(starts, "cpu")), dict(out=out[:-1])):
+        with pytest.raises(ValueError):
+            a8.decode_step_kv8(rows.to(cuda), _ints(lens, cuda), **{**call, **bad})
+    with pytest.raises(ValueError):
+        a8.decode_step_kv8(rows.to(cuda).view(1, n, 2048), _ints(lens, cuda), **call)
+    if norm_rope:
+        runner = a8.PagedDecodeAttentionKV8(cache, kw["gamma_q"], kw["gamma_k"], n, 256)
+        for t, was in zip(cache.kv8().values(), kept):
+            t.copy_(was)
+        got = runner.step(0, rows.to(cuda), _ints(lens, cuda), cache.block_tables(), chunk_lens=_ints(chunk, cuda),
+                          row_start=kw["row_start"], max_tokens=top)
+        runner.check()
+        assert torch.equal(got, out)
+        with pytest.raises(ValueError, match="rows"):
+            runner.step(0, torch.zeros(n + 1, 2048, dtype=BF16, device=cuda), _ints(lens, cuda), cache.block_tables(),
+                        row_start=kw["row_start"], max_tokens=top)
+
+
 def test_prefill_packed_with_a_loose_bound(cuda):
     """max_tokens may be any bound of the chunks."""
     a8, _, _ = _mods()
