@@ -1229,7 +1229,7 @@ constexpr int kPfThreads = 7 * 32;
 constexpr int kPfTmemCols = 256;             // S at columns 0 and 64, O at 128, P at 192 and 224
 constexpr int kPfOperand = kBlock * kDim * 2;
 constexpr int kPfMaxSplit = 32;
-constexpr int kPfSortMax = 128;              // sequences that are started longest first
+constexpr int kPfSortMax = 128;              // sequences whose tiles are started longest first
 constexpr int kPfMaxParts = 320;             // CTAs of a split launch
 constexpr uint32_t kPfIdesc = (1u << 4) | (8u << 17) | (8u << 24);  // f32 <- f16, M 128, N 64, both K-major
 
@@ -1265,6 +1265,8 @@ struct PrefillArgs {
   int num_blocks;
   float scale_log2;
   uint16_t *out;
+  int batch, tiles;      // tiles: of the longest chunk
+  bool sorted;           // jobs by their blocks, not by sequence
   int nsplit;
   PrefillState *parts;   // [query tile][nsplit]
   int32_t *err;
@@ -1295,6 +1297,76 @@ __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0
   return true;
 }
 
+// One warp: the job-th query tile of the batch, the one with the most blocks
+// first (equal ones by sequence): {sequence, tile}, or -1 when there are fewer.
+// Tile t of a sequence with p cached blocks (the last one included) has p + t + 1
+// blocks, its last tile those of the whole length, so the tiles with more than
+// x blocks are counted without a loop over them, and x is found by bisection.
+__device__ void prefill_job(const PrefillArgs &a, int job, int *chosen) {
+  const int lane = threadIdx.x & 31;
+  constexpr int kGroups = kPfSortMax / 32;
+  const int groups = (a.batch + 31) / 32;
+  int held[kGroups], tiles[kGroups], all[kGroups];
+  int top = 0;
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    const int b = i * 32 + lane;
+    held[i] = tiles[i] = 0;
+    if (b < a.batch) {
+      held[i] = a.past_lens[b];
+      tiles[i] = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    PrefillTile t;
+    const int chunk = tiles[i];
+    const bool there = chunk > 0 && prefill_tile(a, i * 32 + lane, 0, job == 0, t);
+    all[i] = there ? (held[i] + chunk - 1) / kBlock + 1 : 0;
+    held[i] = there ? (held[i] + kBlock - 1) / kBlock : 0;
+    tiles[i] = there ? (chunk + kBlock - 1) / kBlock : 0;
+    top = max(top, all[i]);
+  }
+  auto above = [&](int i, int x) { return max(0, tiles[i] - 1 - max(0, x - held[i])) + (all[i] > x ? 1 : 0); };
+  auto count = [&](int x) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      if (i < groups) n += above(i, x);
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(n)));
+  };
+  // the smallest x with at most `job` tiles above it: the job's blocks
+  int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(top)));
+  if (count(0) <= job) {
+    if (lane < 2) chosen[lane] = -1;
+    return;
+  }
+  while (hi - lo > 1) {  // above lo: more than `job` tiles, above hi: not
+    const int x = lo + (hi - lo) / 2;
+    if (count(x) <= job) hi = x;
+    else lo = x;
+  }
+  int skip = job - count(hi);  // of the tiles with hi blocks, which one
+#pragma unroll
+  for (int i = 0; i < kGroups; ++i) {
+    if (i >= groups) break;
+    const int mine = above(i, hi - 1) - above(i, hi);
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    const int before = upto - mine;
+    if (skip >= before && skip < upto) {
+      // the last tile first, then the one before it
+      chosen[0] = i * 32 + lane;
+      chosen[1] = skip == before && all[i] == hi ? tiles[i] - 1 : hi - 1 - held[i];
+    }
+    skip -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
 __device__ __forceinline__ float fmax3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -1302,45 +1374,19 @@ __device__ __forceinline__ float fmax3(float x, float y, float z) {
 }
 
 __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const PrefillArgs a) {
-  const int h = blockIdx.y;
-  const int rank = static_cast<int>(blockIdx.z) / a.nsplit, split = static_cast<int>(blockIdx.z) - rank * a.nsplit;
-  // the last tiles see the most keys: they start first
-  const int tile = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x), t0 = tile * kBlock;
+  // grid: job (a query tile, in the order they start), its parts, its heads
+  const int h = static_cast<int>(blockIdx.x) % kHkv, part = static_cast<int>(blockIdx.x) / kHkv;
+  const int job = part / a.nsplit, split = part - job * a.nsplit;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // .. and the longest sequences: CTAs start in the order of blockIdx, so the
-  // launch does not end on one that came late
-  int b = rank;
-  const int batch = static_cast<int>(gridDim.z) / a.nsplit;
-  if (batch > 1 && batch <= kPfSortMax) {
-    __shared__ int keys[kPfSortMax];
-    __shared__ int chosen;
-    for (int i = tid; i < batch; i += kPfThreads) keys[i] = a.past_lens[i] + (a.chunk_lens ? a.chunk_lens[i] : a.tokens);
-    __syncthreads();
-    for (int i = tid; i < batch; i += kPfThreads) {
-      const int mine = keys[i];
-      int before = 0;
-      for (int q = 0; q < batch; ++q) before += keys[q] > mine || (keys[q] == mine && q < i);
-      if (before == rank) chosen = i;
-    }
-    __syncthreads();
-    b = chosen;
-  }
-  PrefillTile pt;
-  if (!prefill_tile(a, b, t0, tid == 0, pt) || split >= pt.parts) return;
-  const int past = pt.past, rows_t = pt.rows, last_key = past + t0 + rows_t - 1;
-  const int64_t row0 = pt.row;
-  // this CTA's blocks [j0, j0 + nblk)
-  const int j0 = split * pt.per, nblk = min(pt.per, pt.blocks - j0);
-
   extern __shared__ uint8_t smem_raw[];
   uint8_t *sq = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *ring = sq + 2 * kPfOperand;                   // K stages, then V stages
   uint8_t *raw = ring + 2 * kPfStages * kPfOperand;      // codes of K, then of V
   PrefillTail *tail = reinterpret_cast<PrefillTail *>(raw + 2 * kPfRaw * kTile);
 
-  if (tid == 0) {
+  if (tid == 4 * 32) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
 #pragma unroll
@@ -1359,45 +1405,35 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     tail->abort = 0;
     mbar_fence_init();
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
-                 "n"(kPfTmemCols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  // the last tiles of a sequence see the most keys: they start first
+  int b = job / a.tiles, tile = a.tiles - 1 - (job - b * a.tiles);
+  if (a.sorted) {
+    __shared__ int chosen[2];
+    if (warp == 0) prefill_job(a, job, chosen);
+    __syncthreads();
+    b = chosen[0];
+    tile = chosen[1];
+    if (b < 0) return;
+  } else {
+    __syncthreads();
   }
-  // query rows: row r = (head of the pair) * 64 + token, its largest value at 2^8 in f16
-  float factor = 0.f;
-  if (tid < 2 * kBlock) {
-    const int hl = tid >> 6, t = tid & 63;
-    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (row0 + t) * a.q_stride + (2 * h + hl) * kDim);
-    uint4 w[8];
-    float big = 0.f;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      w[c] = t < rows_t ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-      float y[8];
-      unpack8(w[c], y);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e]));
-    }
-    int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
-    e = e < -100 ? -100 : e;
-    const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
-    factor = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      float y[8];
-      unpack8(w[c], y);
-      *reinterpret_cast<uint4 *>(sq + tid * 128 + ((c ^ (tid & 7)) << 4)) =
-          make_uint4(pack_f16x2(y[0] * up, y[1] * up), pack_f16x2(y[2] * up, y[3] * up),
-                     pack_f16x2(y[4] * up, y[5] * up), pack_f16x2(y[6] * up, y[7] * up));
-    }
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  tmem_fence_before();
-  __syncthreads();
-  tmem_fence_after();
-  const uint32_t tmem = tail->tmem;
+  const int t0 = tile * kBlock;
+  PrefillTile pt;
+  if (!prefill_tile(a, b, t0, tid == 0, pt) || split >= pt.parts) return;
+  const int past = pt.past, rows_t = pt.rows, last_key = past + t0 + rows_t - 1;
+  const int64_t row0 = pt.row;
+  // this CTA's blocks [j0, j0 + nblk)
+  const int j0 = split * pt.per, nblk = min(pt.per, pt.blocks - j0);
 
+  // The warps of K and V start at once; the others meet when the query is in
+  // shared memory and the tensor memory allocated.
+  auto meet = [&]() -> uint32_t {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tmem_fence_before();
+    asm volatile("bar.sync 1, 160;" ::: "memory");
+    tmem_fence_after();
+    return tail->tmem;
+  };
   if (warp >= 5) {
     // ---------------- K (warp 5) and V (warp 6): codes in, f16 operands out
     const int which = warp - 5;
@@ -1478,6 +1514,10 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     }
   } else if (warp == 4) {
     // ---------------- products: S_0, S_1, then per block P_j . V_j and S_{j+2}
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
+                 "n"(kPfTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    const uint32_t tmem = meet();
     if (lane == 0) {
       auto issue_s = [&](int j) -> bool {
         const int s = j % kPfStages;
@@ -1523,7 +1563,6 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     const int hl = tid >> 6, t = tid & 63;
     const bool row_ok = t < rows_t;
     const int qpos = past + t0 + t;
-    const uint32_t trow = tmem + (static_cast<uint32_t>(32 * warp) << 16);
     float m = kUnset, mo = kUnset, l = 0.f;
     bool ok = true;
     // decided for the whole warp: the tensor memory accesses are warp-collective
@@ -1540,6 +1579,34 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     };
     int64_t id = pool_tile(lane);
     float2 scale = make_float2(__ldcg(a.k_scale + id), __ldcg(a.v_scale + id)), scale_next = scale;
+    // query rows: row r = (head of the pair) * 64 + token, its largest value at 2^8 in f16
+    float factor = 0.f;
+    {
+      const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (row0 + t) * a.q_stride + (2 * h + hl) * kDim);
+      uint4 w[8];
+      float big = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        w[c] = t < rows_t ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+        float y[8];
+        unpack8(w[c], y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e]));
+      }
+      int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+      e = e < -100 ? -100 : e;
+      const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
+      factor = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float y[8];
+        unpack8(w[c], y);
+        *reinterpret_cast<uint4 *>(sq + tid * 128 + ((c ^ (tid & 7)) << 4)) =
+            make_uint4(pack_f16x2(y[0] * up, y[1] * up), pack_f16x2(y[2] * up, y[3] * up),
+                       pack_f16x2(y[4] * up, y[5] * up), pack_f16x2(y[6] * up, y[7] * up));
+      }
+    }
+    const uint32_t trow = meet() + (static_cast<uint32_t>(32 * warp) << 16);
     for (int j = 0; j < nblk; ++j) {
       if (!warp_wait(smem_u32(&tail->sbar[j & 1]), (j >> 1) & 1)) {
         ok = false;
@@ -1651,7 +1718,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       const float unit = ex2(mo - m);  // the output in units of 2^m, as the sum
       if (stop) {
       } else if (pt.parts > 1) {
-        PrefillState *st = a.parts + ((static_cast<int64_t>(b) * gridDim.x + tile) * kHkv + h) * a.nsplit + split;
+        PrefillState *st = a.parts + ((static_cast<int64_t>(b) * a.tiles + tile) * kHkv + h) * a.nsplit + split;
         float4 *dst = reinterpret_cast<float4 *>(st->o[tid]);
 #pragma unroll
         for (int c = 0; c < 64; c += 4)
@@ -1675,9 +1742,9 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
   }
   tmem_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 4) {
     tmem_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kPfTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tail->tmem), "n"(kPfTmemCols));
   }
 }
 
@@ -1750,7 +1817,7 @@ int launch_prefill(PrefillArgs a, int batch, int max_blocks, cudaStream_t st) {
   if (!prefill_ready()) return fail(B2_ERR_CUDA, "cannot set the prefill kernel's shared memory size");
   // (no chunk is longer than its table; longer ones are refused by their first tile)
   const int64_t longest = a.tokens < static_cast<int64_t>(max_blocks) * kBlock ? a.tokens : static_cast<int64_t>(max_blocks) * kBlock;
-  const int tiles = static_cast<int>((longest + kBlock - 1) / kBlock);
+  const int tiles = a.tiles = static_cast<int>((longest + kBlock - 1) / kBlock);
   const int64_t ctas = static_cast<int64_t>(tiles) * kHkv * batch;
   // Split the keys when the tiles leave SMs without a CTA: about two CTAs per
   // SM, of at least 4 blocks each (as far as the table's width tells).
@@ -1763,7 +1830,11 @@ int launch_prefill(PrefillArgs a, int batch, int max_blocks, cudaStream_t st) {
     if (n > 1) a.nsplit = static_cast<int>(n);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles), kHkv, static_cast<unsigned>(batch * a.nsplit));
+  // More CTAs than start at once: the longest tiles first, so that the launch
+  // does not end on one that came late.
+  a.sorted = a.batch > 1 && a.batch <= kPfSortMax && ctas > 2 * sm_count();
+  if (ctas * a.nsplit > 0x7fffffff) return fail(B2_ERR_ARG, "batch * tokens too large");
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * a.nsplit));
   cfg.blockDim = dim3(kPfThreads);
   cfg.dynamicSmemBytes = kPfSmem;
   cfg.stream = st;
@@ -1914,7 +1985,7 @@ extern "C" int b2_kv8_prefill_attn(const uint16_t *q, int64_t q_stride, int32_t 
     return fail(B2_ERR_ARG, "workspace must be 16-byte aligned and hold b2_kv8_workspace_bytes()");
   if (!(scale > 0.f)) return fail(B2_ERR_ARG, "scale must be positive");
   PrefillArgs a{q, q_stride, rows, row_start, past_lens, chunk_lens, tokens, block_tables, max_blocks_per_seq,
-                k_pool, v_pool, k_scale, v_scale, num_blocks, scale * 1.4426950408889634f, out, 1,
+                k_pool, v_pool, k_scale, v_scale, num_blocks, scale * 1.4426950408889634f, out, batch, 0, false, 1,
                 reinterpret_cast<PrefillState *>(static_cast<char *>(workspace) + kStepBytes), dev_err,
                 b2_wait_limit_ns()};
   return launch_prefill(a, batch, max_blocks_per_seq, static_cast<cudaStream_t>(stream));
