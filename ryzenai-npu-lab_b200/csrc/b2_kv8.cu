@@ -1279,91 +1279,108 @@ struct PrefillTile {
   int past, rows, blocks, per, parts;
   int64_t row;
 };
+__device__ __forceinline__ bool prefill_fits(const PrefillArgs &a, int past, int chunk, int64_t row) {
+  return past >= 0 && chunk <= a.tokens && static_cast<int64_t>(past) + chunk <= static_cast<int64_t>(a.max_blocks) * kBlock &&
+         row >= 0 && row + chunk <= a.rows;
+}
+__device__ __forceinline__ void prefill_blocks(const PrefillArgs &a, int past, int chunk, int64_t row, int t0,
+                                               PrefillTile &t) {
+  t.past = past;
+  t.row = row + t0;
+  t.rows = min(kBlock, chunk - t0);
+  t.blocks = (past + t0 + t.rows - 1) / kBlock + 1;
+  t.per = (t.blocks + a.nsplit - 1) / a.nsplit;
+  t.parts = (t.blocks + t.per - 1) / t.per;
+}
 __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0, bool report, PrefillTile &t) {
   const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
   if (t0 >= chunk) return false;
-  t.past = a.past_lens[b];
-  t.row = a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens;
-  if (t.past < 0 || chunk > a.tokens || static_cast<int64_t>(t.past) + chunk > static_cast<int64_t>(a.max_blocks) * kBlock ||
-      t.row < 0 || t.row + chunk > a.rows) {
+  const int past = a.past_lens[b];
+  const int64_t row = a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens;
+  if (!prefill_fits(a, past, chunk, row)) {
     if (report) atomicOr(a.err, B2_DEV_BAD_LENGTH);
     return false;
   }
-  t.row += t0;
-  t.rows = min(kBlock, chunk - t0);
-  t.blocks = (t.past + t0 + t.rows - 1) / kBlock + 1;
-  t.per = (t.blocks + a.nsplit - 1) / a.nsplit;
-  t.parts = (t.blocks + t.per - 1) / t.per;
+  prefill_blocks(a, past, chunk, row, t0, t);
   return true;
 }
 
+struct PrefillJob {
+  int b, tile, past, chunk;  // b < 0: none
+  int64_t row;
+};
 // One warp: the job-th query tile of the batch, the one with the most blocks
-// first (equal ones by sequence): {sequence, tile}, or -1 when there are fewer.
+// first (equal ones by sequence).
 // Tile t of a sequence with p cached blocks (the last one included) has p + t + 1
 // blocks, its last tile those of the whole length, so the tiles with more than
-// x blocks are counted without a loop over them, and x is found by bisection.
-__device__ void prefill_job(const PrefillArgs &a, int job, int *chosen) {
+// x blocks are counted without a loop over them, and x is found by search.
+__device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
   const int lane = threadIdx.x & 31;
   constexpr int kGroups = kPfSortMax / 32;
   const int groups = (a.batch + 31) / 32;
-  int held[kGroups], tiles[kGroups], all[kGroups];
-  int top = 0;
+  int past[kGroups], chunk[kGroups];
+  int64_t row[kGroups];
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int b = i * 32 + lane;
-    held[i] = tiles[i] = 0;
-    if (b < a.batch) {
-      held[i] = a.past_lens[b];
-      tiles[i] = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
-    }
+    const bool there = b < a.batch;
+    past[i] = there ? a.past_lens[b] : 0;
+    chunk[i] = there ? (a.chunk_lens ? a.chunk_lens[b] : a.tokens) : 0;
+    row[i] = !a.row_start ? static_cast<int64_t>(b) * a.tokens : there ? a.row_start[b] : 0;
   }
+  int held[kGroups], full[kGroups], all[kGroups];  // blocks cached, tiles before the last, blocks of the last
+  int top = 0, n = 0;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    PrefillTile t;
-    const int chunk = tiles[i];
-    const bool there = chunk > 0 && prefill_tile(a, i * 32 + lane, 0, job == 0, t);
-    all[i] = there ? (held[i] + chunk - 1) / kBlock + 1 : 0;
-    held[i] = there ? (held[i] + kBlock - 1) / kBlock : 0;
-    tiles[i] = there ? (chunk + kBlock - 1) / kBlock : 0;
+    held[i] = full[i] = all[i] = 0;
+    if (chunk[i] <= 0) continue;
+    if (!prefill_fits(a, past[i], chunk[i], row[i])) {
+      if (job == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+      continue;
+    }
+    held[i] = (past[i] + kBlock - 1) / kBlock;
+    full[i] = (chunk[i] + kBlock - 1) / kBlock - 1;
+    all[i] = (past[i] + chunk[i] - 1) / kBlock + 1;
     top = max(top, all[i]);
+    n += full[i] + 1;
   }
-  auto above = [&](int i, int x) { return max(0, tiles[i] - 1 - max(0, x - held[i])) + (all[i] > x ? 1 : 0); };
+  if (static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(n))) <= job) {
+    if (lane == 0) chosen.b = -1;
+    return;
+  }
+  auto above = [&](int i, int x) { return full[i] - min(max(x - held[i], 0), full[i]) + (all[i] > x ? 1 : 0); };
   auto count = [&](int x) {
-    int n = 0;
+    int c = 0;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i)
-      if (i < groups) n += above(i, x);
-    return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(n)));
+      if (i < groups) c += above(i, x);
+    return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c)));
   };
   // the smallest x with at most `job` tiles above it: the job's blocks
   int lo = 0, hi = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(top)));
-  if (count(0) <= job) {
-    if (lane < 2) chosen[lane] = -1;
-    return;
-  }
   while (hi - lo > 1) {  // above lo: more than `job` tiles, above hi: not
-    const int x = lo + (hi - lo) / 2;
-    if (count(x) <= job) hi = x;
-    else lo = x;
+    const int d = (hi - lo + 3) >> 2, x1 = lo + d, x2 = min(x1 + d, hi), x3 = min(x2 + d, hi);
+    const bool p1 = count(x1) <= job, p2 = count(x2) <= job, p3 = count(x3) <= job;
+    lo = p1 ? lo : (p2 ? x1 : (p3 ? x2 : x3));
+    hi = p1 ? x1 : (p2 ? x2 : (p3 ? x3 : hi));
   }
   int skip = job - count(hi);  // of the tiles with hi blocks, which one
+  const unsigned below = (1u << lane) - 1u;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     if (i >= groups) break;
-    const int mine = above(i, hi - 1) - above(i, hi);
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += y;
-    }
-    const int before = upto - mine;
-    if (skip >= before && skip < upto) {
+    const int mine = above(i, hi - 1) - above(i, hi);  // 0, 1 or 2
+    const unsigned one = __ballot_sync(0xffffffffu, mine >= 1), two = __ballot_sync(0xffffffffu, mine == 2);
+    const int before = __popc(one & below) + __popc(two & below);
+    if (skip >= before && skip < before + mine) {
       // the last tile first, then the one before it
-      chosen[0] = i * 32 + lane;
-      chosen[1] = skip == before && all[i] == hi ? tiles[i] - 1 : hi - 1 - held[i];
+      chosen.b = i * 32 + lane;
+      chosen.tile = skip == before && all[i] == hi ? full[i] : hi - 1 - held[i];
+      chosen.past = past[i];
+      chosen.chunk = chunk[i];
+      chosen.row = row[i];
     }
-    skip -= __shfl_sync(0xffffffffu, upto, 31);
+    skip -= __popc(one) + __popc(two);
   }
 }
 
@@ -1407,19 +1424,21 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
   }
   // the last tiles of a sequence see the most keys: they start first
   int b = job / a.tiles, tile = a.tiles - 1 - (job - b * a.tiles);
+  PrefillTile pt;
   if (a.sorted) {
-    __shared__ int chosen[2];
+    __shared__ PrefillJob chosen;
     if (warp == 0) prefill_job(a, job, chosen);
     __syncthreads();
-    b = chosen[0];
-    tile = chosen[1];
+    b = chosen.b;
+    tile = chosen.tile;
     if (b < 0) return;
+    prefill_blocks(a, chosen.past, chosen.chunk, chosen.row, tile * kBlock, pt);
   } else {
     __syncthreads();
+    if (!prefill_tile(a, b, tile * kBlock, tid == 0, pt)) return;
   }
+  if (split >= pt.parts) return;
   const int t0 = tile * kBlock;
-  PrefillTile pt;
-  if (!prefill_tile(a, b, t0, tid == 0, pt) || split >= pt.parts) return;
   const int past = pt.past, rows_t = pt.rows, last_key = past + t0 + rows_t - 1;
   const int64_t row0 = pt.row;
   // this CTA's blocks [j0, j0 + nblk)
