@@ -1294,9 +1294,9 @@ __device__ __forceinline__ void prefill_blocks(const PrefillArgs &a, int past, i
 }
 __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0, bool report, PrefillTile &t) {
   const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
-  if (t0 >= chunk) return false;
   const int past = a.past_lens[b];
   const int64_t row = a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens;
+  if (t0 >= chunk) return false;
   if (!prefill_fits(a, past, chunk, row)) {
     if (report) atomicOr(a.err, B2_DEV_BAD_LENGTH);
     return false;
@@ -1314,10 +1314,9 @@ struct PrefillJob {
 // Tile t of a sequence with p cached blocks (the last one included) has p + t + 1
 // blocks, its last tile those of the whole length, so the tiles with more than
 // x blocks are counted without a loop over them, and x is found by search.
+template <int kGroups>  // of 32 sequences
 __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
   const int lane = threadIdx.x & 31;
-  constexpr int kGroups = kPfSortMax / 32;
-  const int groups = (a.batch + 31) / 32;
   int past[kGroups], chunk[kGroups];
   int64_t row[kGroups];
 #pragma unroll
@@ -1352,8 +1351,7 @@ __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
   auto count = [&](int x) {
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i)
-      if (i < groups) c += above(i, x);
+    for (int i = 0; i < kGroups; ++i) c += above(i, x);
     return static_cast<int>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(c)));
   };
   // the smallest x with at most `job` tiles above it: the job's blocks
@@ -1368,7 +1366,6 @@ __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
   const unsigned below = (1u << lane) - 1u;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
-    if (i >= groups) break;
     const int mine = above(i, hi - 1) - above(i, hi);  // 0, 1 or 2
     const unsigned one = __ballot_sync(0xffffffffu, mine >= 1), two = __ballot_sync(0xffffffffu, mine == 2);
     const int before = __popc(one & below) + __popc(two & below);
@@ -1427,7 +1424,11 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
   PrefillTile pt;
   if (a.sorted) {
     __shared__ PrefillJob chosen;
-    if (warp == 0) prefill_job(a, job, chosen);
+    if (warp == 0) {
+      if (a.batch <= 32) prefill_job<1>(a, job, chosen);
+      else if (a.batch <= 64) prefill_job<2>(a, job, chosen);
+      else prefill_job<kPfSortMax / 32>(a, job, chosen);
+    }
     __syncthreads();
     b = chosen.b;
     tile = chosen.tile;

@@ -447,6 +447,38 @@ def test_step_packed(cuda, top, norm_rope, binding, monkeypatch):
                         row_start=kw["row_start"], max_tokens=top)
 
 
+@pytest.mark.parametrize("n", [9, 33, 64, 65, 128, 129])
+def test_prefill_packed_many_ragged(cuda, n):
+    """More query tiles than start at once: sorted by their blocks, or (more than 128 sequences) as they come; a
+    sequence whose chunk passes max_tokens is refused, the others are not."""
+    a8, _, lib = _mods()
+    g = torch.Generator().manual_seed(n)
+    top = 700 if n < 30 else 140
+    lens = torch.randint(0, 300, (n,), generator=g).tolist()
+    chunk = torch.randint(0, top + 1, (n,), generator=g).tolist()
+    chunk[0], chunk[1], chunk[n // 2], lens[2] = 0, top, 64, 64
+    starts = [sum(chunk[:b]) for b in range(n)]
+    cache, ref = _build(lens, cuda, seed=n, room=top + 1)
+    rows = _rows(sum(chunk), n, cuda)
+    slots = torch.full((sum(chunk),), -1, dtype=I32)
+    tables = cache.block_tables().cpu()
+    for b in range(n):
+        for t in range(chunk[b]):
+            p = lens[b] + t
+            slots[starts[b] + t] = int(tables[b, p // 64]) * 64 + p % 64
+    kw = dict(row_start=_ints(starts, cuda), max_tokens=top, slots=slots.to(cuda))
+    out = _prefill(cache, rows, lens, cuda, chunk, **kw)
+    want = out.clone()
+    _check_rows(cache, ref, rows, out, lens, starts, chunk)
+    err, out = _err(cuda), torch.zeros_like(out)
+    bad = [top + 1 if b == 1 else c for b, c in enumerate(chunk)]
+    a8.prefill_kv8(rows.to(cuda), _ints(lens, cuda), block_tables=cache.block_tables(), dev_err=err, out=out,
+                   workspace=a8.workspace_kv8(cuda), chunk_lens=_ints(bad, cuda), mode=0, **cache.kv8(), **kw)
+    assert err.item() == lib.B2_DEV_BAD_LENGTH
+    want[starts[1]:starts[1] + top] = 0
+    assert torch.equal(out, want)
+
+
 def test_prefill_packed_with_a_loose_bound(cuda):
     """max_tokens may be any bound of the chunks."""
     a8, _, _ = _mods()
