@@ -178,9 +178,12 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
 // tokens of two V dims, for which shared memory is the transpose.
 //
 // Bound by latency: a run's loads, its codes, its stores (64 x 128 tokens 14 us,
-// 8 of them the loads; 21 tokens 4.9 us).  kWindow 8 spreads few rows over the
-// SMs; 32 keeps the CTAs that hold no run's start from outnumbering the others
-// in long prompts (64: 15-25 % slower there, 8: 10 %).
+// 8 of them the loads; 21 tokens 4.4 us).  A warp takes the runs of its window in
+// turn, so many short runs want kWindow 8 (256 sequences x 4 tokens 7.5 us, with
+// 32 17.9; 128 x 16: 7.5, 9.1), while CTAs that hold no run's start only cost in
+// long prompts (one of 1024 tokens 7.2 us, with 32 5.0; 32 x 32: 7.8, 6.1; 64 x
+// 128 10 % slower, with 64 15-25 %).  Where the rows' runs are not known (slots),
+// up to 1024 rows take 8.
 template <int kWindow>
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const AppendArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -1156,7 +1159,8 @@ int sm_count() {
 }
 
 constexpr int64_t kCounterBytes = kMaxCtas * kMaxStepTokens * 4;
-constexpr int64_t kStepBytes = kCounterBytes + 2 * kMaxCtas * static_cast<int64_t>(sizeof(StepShared<kMaxStepTokens>::State));
+constexpr int64_t kStepBytes =
+    kCounterBytes + 2 * kMaxCtas * static_cast<int64_t>(sizeof(StepShared<kMaxStepTokens>::State));
 
 template <int kT>
 int launch_step(StepArgs a, cudaStream_t st) {
@@ -1213,6 +1217,20 @@ int launch_step(StepArgs a, cudaStream_t st) {
 // them as 128-byte-swizzled operands.  V is stored dim-major, so both B operands
 // are K-major.  S and P are double-buffered, as the operands' rings are, so
 // conversion, products and softmax of different blocks overlap.
+//
+// 64 sequences, 128 new tokens over 128-8192 cached: 286 us with the append (14),
+// against 84 us of products at the matrix rate and 50 us of bytes.  Profiled:
+// exponentials 52 % of their pipe, matrix pipe 25 %, DRAM 13 %, issue 50 %: what
+// bounds it is the chain of a block (S, 64 scores to registers, maximum, 64
+// exponentials, P to tensor memory), about 1.1 us, of which two CTAs per SM run
+// side by side.  Three CTAs per SM with half the stages (344 us against 331 then),
+// four with single buffers (441) and more registers for the softmax warps
+// (setmaxnreg, 340) were slower.  The rest is a CTA's start, a row of dependent
+// loads under load, about 5 us: reading a tile's lengths a second time after the
+// search for it cost 21 us in all, starting K and V only behind the query 5.
+//
+// A launch of more CTAs than start at once runs its query tiles longest first;
+// as they come: 376 us against 324 at that step.
 //
 // The scales never touch the operands: a row's scores are S * (q factor * k
 // scale), and P is p * g with g = v scale * 2^(m - mo), the references m (of
@@ -1952,7 +1970,8 @@ extern "C" int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t ro
                max_blocks_per_seq, gamma_q, gamma_k, eps, rope_cos, rope_sin, rope_rows, k_pool, v_pool,
                k_scale, v_scale, num_blocks, q_out, mode, dev_err};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return rows <= 1024 ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
+  const bool short_runs = slots ? rows <= 1024 : tokens <= 16;
+  return short_runs ? launch_append<8>(a, st) : launch_append<kMaxWindow>(a, st);
 }
 
 extern "C" int b2_kv8_decode_step(const uint16_t *qkv, int64_t row_stride, int32_t rows, const int32_t *row_start,

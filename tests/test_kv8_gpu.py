@@ -73,6 +73,21 @@ def test_append_codes_and_scales(cuda, past, n, by_slots):
     assert ref.same_as(cache.kv8())
 
 
+@pytest.mark.parametrize("b,n", [(130, 16), (67, 17), (300, 3)])
+def test_append_of_many_short_runs(cuda, b, n):
+    a8, pc, lib = _mods()
+    lens = [(7 * i) % 70 for i in range(b)]
+    cache, ref = _build(lens, cuda, seed=n, room=n)
+    rows, err, tables = _rows(b * n, n, cuda).view(b, n, 2048), _err(cuda), cache.block_tables()
+    a8.append_kv8(rows.to(cuda), past_lens=_ints(lens, cuda), block_tables=tables, dev_err=err, mode=lib.B2_STORE_KV,
+                  **cache.kv8())
+    for i, p in enumerate(lens):
+        _, k, v = ora.split(rows[i])
+        ora.append(ref, tables[i].cpu(), p, k, v)
+    assert err.item() == 0
+    assert ref.same_as(cache.kv8())
+
+
 def test_append_skips_negative_slots_and_strange_values(cuda):
     """Negative slots are padding; zeros, tiny, huge, infinite and NaN values have their codes and scales."""
     a8, _, lib = _mods()

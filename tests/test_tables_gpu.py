@@ -65,6 +65,12 @@ def test_extend(cuda, b, top, tight, packed, in_place):
     assert got == want
 
 
+@pytest.mark.parametrize("b,top,packed", [(293, 1801, False), (911, 1301, True), (3, 200001, True)])
+def test_extend_many_rows(cuda, b, top, packed):
+    """Above half a million rows: several per thread, requests that end inside a thread's rows."""
+    test_extend(cuda, b, top, False, packed, False)
+
+
 def test_extend_refuses_what_cannot_be(cuda):
     """Negative lengths, a full row, rows behind the last one, more tokens than a padded row has: refused, the
     others served."""
