@@ -99,6 +99,7 @@ int64_t b2_kv8_workspace_bytes(void);
  * row_start  int32 [batch]: the row of a sequence's first token (packed
  *            prompts); NULL: b * tokens.
  * chunk_lens int32 [batch], 0 .. tokens; NULL: tokens.
+ * tokens     the longest chunk; batch * ceil(tokens / 64) * 8 < 2^31.
  * rows       rows of q and out; a sequence that would leave them is refused
  *            (B2_DEV_BAD_LENGTH).
  * out        bf16 [rows][16][64]; rows of no token are left as they were.

@@ -325,7 +325,7 @@ class PagedDecodeAttentionKV8:
         """qkv bf16 [B, W] (one token per sequence), [B, T, W] or, with row_start
         and max_tokens, packed [rows, W] raw projections; returns the contexts
         [B, 16, 64], [B, T, 16, 64] or [rows, 16, 64]."""
-        if row_start is not None:
+        if row_start is not None or max_tokens is not None:
             if out is None:
                 if qkv.shape[0] > self.out.shape[0]:
                     raise ValueError(f"{qkv.shape[0]} rows > max_batch x max_tokens {self.out.shape[0]}")

@@ -182,6 +182,10 @@ class PagedKVCache8(PagedKVCache):
         v        float8_e4m3fn [layers, num_blocks, 8, 64 dims, 64 tokens]
         k_scale, v_scale       float32 [layers, num_blocks, 8]
 
+    A block's scale follows its largest value and never falls while the block
+    holds tokens: after a shorter length (drafted tokens that were rejected) the
+    next append keeps the scale that they raised.
+
     attention_kv8 appends to it and attends over it; the bf16 kernels refuse
     it.  Block allocation and tables are PagedKVCache's."""
 

@@ -457,9 +457,39 @@ def test_step_packed(cuda, top, norm_rope, binding, monkeypatch):
                           row_start=kw["row_start"], max_tokens=top)
         runner.check()
         assert torch.equal(got, out)
+        with pytest.raises(ValueError, match="row_start"):
+            runner.step(0, rows.to(cuda), _ints(lens, cuda), cache.block_tables(), max_tokens=top)
         with pytest.raises(ValueError, match="rows"):
             runner.step(0, torch.zeros(n + 1, 2048, dtype=BF16, device=cuda), _ints(lens, cuda), cache.block_tables(),
                         row_start=kw["row_start"], max_tokens=top)
+
+
+def test_step_packed_of_many_sequences(cuda):
+    """More sequences than one launch takes, some without a new token: as the padded call."""
+    a8, _, lib = _mods()
+    n = 2100
+    lens = [(11 * i) % 90 for i in range(n)]
+    chunk = [(i % 5 > 0) + (i % 7 == 0) for i in range(n)]
+    starts = [sum(chunk[:b]) for b in range(n)]
+    cache, _ = _build(lens, cuda, seed=8, room=3)
+    kept = [t.clone() for t in cache.kv8().values()]
+    rows = _rows(sum(chunk), 8, cuda)
+    padded = torch.zeros(n, 2, 2048, dtype=BF16)
+    for b in range(n):
+        padded[b, :chunk[b]] = rows[starts[b]:starts[b] + chunk[b]]
+    want = _step(cache, padded, lens, cuda, chunk)
+    after = [t.clone().view(torch.uint8) for t in cache.kv8().values()]
+    for t, was in zip(cache.kv8().values(), kept):
+        t.copy_(was)
+    out = torch.full((sum(chunk), 16, 64), -7.0, dtype=BF16, device=cuda)
+    err = _err(cuda)
+    a8.decode_step_kv8(rows.to(cuda), _ints(lens, cuda), block_tables=cache.block_tables(), out=out, dev_err=err,
+                       workspace=a8.workspace_kv8(cuda), chunk_lens=_ints(chunk, cuda), mode=lib.B2_STORE_KV,
+                       row_start=_ints(starts, cuda), max_tokens=2, **cache.kv8())
+    assert err.item() == 0
+    assert all(torch.equal(x.view(torch.uint8), y) for x, y in zip(cache.kv8().values(), after))
+    there = torch.arange(2)[None] < torch.tensor(chunk)[:, None]
+    assert torch.equal(out, want[there.to(cuda)])
 
 
 @pytest.mark.parametrize("n", [9, 33, 64, 65, 128, 129])
