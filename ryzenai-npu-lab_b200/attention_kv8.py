@@ -28,7 +28,7 @@ NORM_ROPE_STORE = _lib.B2_NORM_QK | _lib.B2_ROPE_QK | _lib.B2_STORE_KV
 
 # The smallest calls are bound by the host.  The native binding (_b2torch, built
 # against the installed torch) checks a call's tensors and makes the library call
-# in about 2 us; where it is not built, or says None to an argument, the checks
+# in one go, in half the time; where it is not built, or says None to an argument, the checks
 # below do the same: each is one comparison of what the tensor says about itself
 # (its device by index), and the slow path that words the refusal is taken only
 # when one fails.
@@ -246,7 +246,8 @@ def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Ten
     if native is not None and qkv.dim() >= 2 and qkv.shape[-1] >= QKV_WIDTH:
         q_buf = None
         if mode & (_lib.B2_NORM_QK | _lib.B2_ROPE_QK):
-            q_buf = torch.empty(qkv.numel() // qkv.shape[-1], HQ, D, dtype=_BF16, device=qkv.device)
+            with torch.cuda.stream(stream):     # freed behind the kernels that use it
+                q_buf = torch.empty(qkv.numel() // qkv.shape[-1], HQ, D, dtype=_BF16, device=qkv.device)
         rc = native.prefill(qkv, past_lens, k_pool, v_pool, k_scale, v_scale, block_tables, out, workspace, dev_err,
                             chunk_lens, gamma_q, gamma_k, cos, sin, mode, eps, scale, raw, row_start, max_tokens, slots,
                             positions, q_buf)
@@ -273,7 +274,8 @@ def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Ten
         tokens = int(max_tokens)
         shape = (rows, HQ, D)
     if out is None:
-        out = torch.zeros(shape, dtype=_BF16, device=qkv.device)
+        with torch.cuda.stream(stream):
+            out = torch.zeros(shape, dtype=_BF16, device=qkv.device)
     to = _is(out, "out", _BF16, qkv, index, shape)
     cache = _need_cache(k_pool, v_pool, k_scale, v_scale, qkv, index)
     work = _need_workspace(workspace, qkv, index)
@@ -283,7 +285,8 @@ def prefill_kv8(qkv: torch.Tensor, past_lens: torch.Tensor, *, k_pool: torch.Ten
     place = None if positions is None else _is(positions, "positions", _I32, qkv, index, (rows,))
     qk = _need_qk(mode, gamma_q, gamma_k, eps, cos, sin, qkv, index)
     turned = mode & (_lib.B2_NORM_QK | _lib.B2_ROPE_QK)
-    q_buf = torch.empty(rows, HQ, D, dtype=_BF16, device=qkv.device) if turned else None
+    with torch.cuda.stream(stream):
+        q_buf = torch.empty(rows, HQ, D, dtype=_BF16, device=qkv.device) if turned else None
     if mode:
         _launch("b2_kv8_append", index, stream, q, width, rows, slot, place, past, chunk, tokens, tables, table_width,
                 *qk, *cache, None if q_buf is None else q_buf.data_ptr(), mode, err)

@@ -766,6 +766,32 @@ def test_native_binding_and_python_checks_agree(cuda, binding, monkeypatch):
         dev.plan(_ints([1, 1, 1], cuda), rows=3)
 
 
+@pytest.mark.parametrize("binding", [True, False])
+@pytest.mark.parametrize("given", [True, False])
+def test_prefill_on_another_stream(cuda, binding, given, monkeypatch):
+    """The call's own buffers belong to the stream it runs on: work that the current stream is given meanwhile
+    does not get them."""
+    a8, _, lib = _mods()
+    if not binding:
+        monkeypatch.setattr(a8, "_b2torch", None)
+    cache, _ = _build([70, 3], cuda, seed=19, room=80)
+    w = orc.attention_weights(6)
+    cos, sin = load_pkg("rope").rope_table(256, device=cuda)
+    rows, past = _rows(140, 19, cuda).view(2, 70, 2048).to(cuda), _ints([70, 3], cuda)
+    args = dict(block_tables=cache.block_tables(), workspace=a8.workspace_kv8(cuda), dev_err=_err(cuda),
+                gamma_q=w["q_gamma"].to(cuda), gamma_k=w["k_gamma"].to(cuda), cos=cos, sin=sin, mode=7, **cache.kv8())
+    want = a8.prefill_kv8(rows, past, **args)
+    out = torch.zeros_like(want) if given else None
+    side = torch.cuda.Stream(cuda)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+    got = a8.prefill_kv8(rows, past, out=out, stream=side, **args)
+    junk = [torch.full((140, 16, 64), float("nan"), dtype=BF16, device=cuda) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and args["dev_err"].item() == 0 and bool(junk[0].isnan().all())
+
+
 def test_refuses_host_tensors(cuda):
     """Tensors that are all on the host never reach the library."""
     a8, pc, lib = _mods()
