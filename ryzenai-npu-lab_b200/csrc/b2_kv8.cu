@@ -1225,7 +1225,9 @@ int launch_step(StepArgs a, cudaStream_t st) {
 // exponentials, P to tensor memory), about 1.1 us, of which two CTAs per SM run
 // side by side.  Three CTAs per SM with half the stages (344 us against 331 then),
 // four with single buffers (441) and more registers for the softmax warps
-// (setmaxnreg, 340) were slower.  The rest is a CTA's start, a row of dependent
+// (setmaxnreg, 340) were slower, and so were two sets of softmax warps on
+// alternate blocks, with 80 registers and P in the place of S (328 against 286:
+// each waits for its products).  The rest is a CTA's start, a row of dependent
 // loads under load, about 5 us: reading a tile's lengths a second time after the
 // search for it cost 21 us in all, starting K and V only behind the query 5.
 //
