@@ -48,7 +48,9 @@ extern "C" {
  *              positions int32 [rows] are the RoPE positions (B2_ROPE_QK).
  *   slots NULL rows = batch * tokens, row b * tokens + t at position
  *              past_lens[b] + t, for t < chunk_lens[b] (NULL: tokens), through
- *              block_tables [batch][max_blocks_per_seq].
+ *              block_tables [batch][max_blocks_per_seq].  A sequence with
+ *              a negative length, more than `tokens` new tokens or more tokens
+ *              than its table holds is refused whole (B2_DEV_BAD_LENGTH).
  * q_out      bf16 [rows][16][64] normalised and rotated query, or NULL; rows
  *            that are skipped are left as they were.
  */

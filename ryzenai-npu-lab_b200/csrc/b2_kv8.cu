@@ -147,16 +147,14 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
   }
   const int b = row / a.tokens, t = row - b * a.tokens;
   const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
-  if (chunk > a.tokens) {
+  const int64_t past = a.past_lens[b], pos = past + t;
+  if (chunk == 0) return kNoSlot;
+  // lengths that do not fit refuse the sequence whole, as the attention does: its cached tokens stay as they are
+  if (past < 0 || chunk < 0 || chunk > a.tokens || past + chunk > static_cast<int64_t>(a.max_blocks) * kBlock) {
     flag |= B2_DEV_BAD_LENGTH;
     return kNoSlot;
   }
   if (t >= chunk) return kNoSlot;
-  const int64_t pos = static_cast<int64_t>(a.past_lens[b]) + t;
-  if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) {
-    flag |= B2_DEV_BAD_LENGTH;
-    return kNoSlot;
-  }
   position = static_cast<int>(pos);
   if (!(a.mode & B2_STORE_KV)) return 0;
   const int blk = a.block_tables[static_cast<int64_t>(b) * a.max_blocks + pos / kBlock];
