@@ -1298,7 +1298,8 @@ struct PrefillTile {
   int64_t row;
 };
 __device__ __forceinline__ bool prefill_fits(const PrefillArgs &a, int past, int chunk, int64_t row) {
-  return past >= 0 && chunk <= a.tokens && static_cast<int64_t>(past) + chunk <= static_cast<int64_t>(a.max_blocks) * kBlock &&
+  return past >= 0 && chunk >= 0 && chunk <= a.tokens &&
+         static_cast<int64_t>(past) + chunk <= static_cast<int64_t>(a.max_blocks) * kBlock &&
          row >= 0 && row + chunk <= a.rows;
 }
 __device__ __forceinline__ void prefill_blocks(const PrefillArgs &a, int past, int chunk, int64_t row, int t0,
@@ -1314,11 +1315,12 @@ __device__ __forceinline__ bool prefill_tile(const PrefillArgs &a, int b, int t0
   const int chunk = a.chunk_lens ? a.chunk_lens[b] : a.tokens;
   const int past = a.past_lens[b];
   const int64_t row = a.row_start ? static_cast<int64_t>(a.row_start[b]) : static_cast<int64_t>(b) * a.tokens;
-  if (t0 >= chunk) return false;
+  if (chunk == 0) return false;
   if (!prefill_fits(a, past, chunk, row)) {
     if (report) atomicOr(a.err, B2_DEV_BAD_LENGTH);
     return false;
   }
+  if (t0 >= chunk) return false;
   prefill_blocks(a, past, chunk, row, t0, t);
   return true;
 }
@@ -1350,7 +1352,7 @@ __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     held[i] = full[i] = all[i] = 0;
-    if (chunk[i] <= 0) continue;
+    if (chunk[i] == 0) continue;
     if (!prefill_fits(a, past[i], chunk[i], row[i])) {
       if (job == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
       continue;

@@ -39,3 +39,20 @@ def test_a_refused_sequence_is_left_as_it_was(cuda, call, past, chunk):
         if call == "prefill":
             ora.check_context(out[b, :n], *ora.attend(ref, tables[b].cpu(), p, q), f"sequence {b}")
     assert ref.same_as(cache.kv8())
+
+
+def test_prefill_flags_a_negative_chunk(cuda):
+    """Packed rows and a batch whose tiles are sorted, too."""
+    a8, _, lib = _mods()
+    for b in (2, 40):
+        cache, _ = _build([30] * b, cuda, seed=203, room=80)
+        rows = _rows(b * 65, 204, cuda).to(cuda)
+        slots = _ints([-1] * (65 * b), cuda)
+        out = torch.full((65 * b, 16, 64), -7.0, dtype=BF16, device=cuda)
+        err = _err(cuda)
+        a8.prefill_kv8(rows, _ints([30] * b, cuda), block_tables=cache.block_tables(), workspace=a8.workspace_kv8(cuda),
+                       dev_err=err, mode=lib.B2_STORE_KV, chunk_lens=_ints([1] * (b - 1) + [-3], cuda),
+                       row_start=_ints([65 * i for i in range(b)], cuda), max_tokens=65, slots=slots, out=out,
+                       **cache.kv8())
+        assert err.item() == lib.B2_DEV_BAD_LENGTH
+        assert bool((out.view(b, 65, 16, 64)[-1] == -7.0).all())
