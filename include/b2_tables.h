@@ -53,7 +53,9 @@ int b2_tables_extend(int32_t *block_tables, int32_t max_blocks_per_seq, const in
 /*
  * The slots and positions alone, from tables whose blocks are there:
  * row_start[b] + t (NULL: b * tokens_per_seq + t) for t < new_lens[b].  With
- * row_start the starts ascend and requests do not overlap.
+ * row_start the starts ascend and requests do not overlap.  A request that
+ * b2_tables_extend would refuse for its lengths, or whose first row is
+ * negative, gets no slot at all (-1) and sets B2_DEV_BAD_LENGTH.
  */
 int b2_slot_map(const int32_t *block_tables, int32_t max_blocks_per_seq, int32_t num_blocks,
                 const int32_t *past_lens, const int32_t *new_lens, const int32_t *row_start, int32_t batch,

@@ -73,7 +73,8 @@ def slot_map(block_tables: torch.Tensor, past_lens: torch.Tensor, new_lens: torc
              stream: torch.cuda.Stream | None = None) -> None:
     """Slots and positions of new_lens[b] tokens behind past_lens[b] from tables
     whose blocks are there (b2_slot_map): rows from row_start[b] on (ascending,
-    not overlapping), or rows b * tokens_per_seq + t."""
+    not overlapping), or rows b * tokens_per_seq + t.  A request whose lengths
+    do not fit gets no slot at all (-1) and is flagged in dev_err."""
     b, width = _table_shape(block_tables)
     rows, index, per_b = slots.numel(), block_tables.get_device(), (b,)
     _launch("b2_slot_map", index, stream,

@@ -81,6 +81,12 @@ struct SlotArgs {
   int32_t *err;  // NULL: faults were reported before
 };
 
+// Request b of a slot map can be placed: as extend_kernel's `bad`, with its first row.
+__device__ __forceinline__ bool request_fits(const SlotArgs &a, int64_t start, int past, int fresh) {
+  return past >= 0 && fresh >= 0 && static_cast<int64_t>(past) + fresh <= static_cast<int64_t>(a.max_blocks) * kBlock &&
+         (a.row_start ? fresh == 0 || (start >= 0 && start + fresh <= a.rows) : fresh <= a.tokens);
+}
+
 // Rows r0 .. r0 + kSlotRows - 1, ascending from request b on (the last one that
 // starts at or before r0): eight rows share the search for their request and
 // leave as 16-byte stores; one row per thread keeps few rows' loads parallel.
@@ -95,7 +101,7 @@ __device__ __forceinline__ void write_rows(const SlotArgs &a, int64_t r0, int b)
     start = !in ? 0 : (kPadded ? static_cast<int64_t>(b) * a.tokens : a.row_start[b]);
     past = in ? a.past[b] : 0;
     fresh = in ? a.fresh[b] : 0;
-    granted = in && (!a.granted || a.granted[b] > 0);
+    granted = in && (a.granted ? a.granted[b] > 0 : request_fits(a, start, past, fresh));
     held_blk = -1;
   };
   request();
@@ -123,10 +129,7 @@ __device__ __forceinline__ void write_rows(const SlotArgs &a, int64_t r0, int b)
     const int64_t pos = past + t;
     position[i] = static_cast<int>(pos);
     if (!granted) continue;
-    if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) {
-      flag |= B2_DEV_BAD_LENGTH;
-      continue;
-    }
+    if (pos < 0 || pos >= static_cast<int64_t>(a.max_blocks) * kBlock) continue;  // (starts that do not ascend)
     const int logical = static_cast<int>(pos / kBlock);
     if (logical != held_blk) {
       blk = a.tables[static_cast<int64_t>(b) * a.max_blocks + logical];
@@ -307,7 +310,13 @@ __global__ void __launch_bounds__(kScanThreads) extend_kernel(const ExtendArgs a
 template <int kSlotRows>
 __global__ void __launch_bounds__(kSlotThreads) slot_kernel(const SlotArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x) * kSlotRows;
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * kSlotThreads + threadIdx.x, r0 = thread * kSlotRows;
+  if (a.err) {  // requests that are refused, whether a row shows them or not
+    bool bad = false;
+    for (int64_t b = thread; b < a.batch; b += static_cast<int64_t>(gridDim.x) * kSlotThreads)
+      bad = bad || !request_fits(a, a.row_start ? a.row_start[b] : b * a.tokens, a.past[b], a.fresh[b]);
+    if (bad) atomicOr(a.err, B2_DEV_BAD_LENGTH);
+  }
   if (r0 < a.rows) find_and_write_rows<kSlotRows>(a, r0);
 }
 

@@ -56,3 +56,44 @@ def test_prefill_flags_a_negative_chunk(cuda):
                        **cache.kv8())
         assert err.item() == lib.B2_DEV_BAD_LENGTH
         assert bool((out.view(b, 65, 16, 64)[-1] == -7.0).all())
+
+
+@pytest.mark.parametrize("many", [False, True])         # one row per thread, eight
+def test_slot_map_refuses_a_request_whole(cuda, many):
+    """Slots of a request whose lengths do not fit are -1, all of them, as extend_tables writes them."""
+    bt, lib = load_pkg("block_tables"), load_pkg("_lib")
+    top = 140000 if many else 40
+    width = (200 + top + 63) // 64
+    tables = torch.arange(5 * width, dtype=I32, device=cuda).view(5, width)
+    end = width * 64
+
+    def run(past, new, starts, rows, tps):
+        slots, positions, err = _ints([9] * rows, cuda), _ints([9] * rows, cuda), _err(cuda)
+        bt.slot_map(tables, _ints(past, cuda), _ints(new, cuda), num_blocks=5 * width, slots=slots, positions=positions,
+                    row_start=None if starts is None else _ints(starts, cuda), tokens_per_seq=tps, dev_err=err)
+        return slots.cpu(), err.item()
+
+    def check(past, new, starts, rows, tps, refused):
+        slots, flags = run(past, new, starts, rows, tps)
+        assert flags == (lib.B2_DEV_BAD_LENGTH if refused else 0)
+        want = torch.full((rows,), -1, dtype=I32)
+        for b in range(5):
+            if b not in refused and new[b] > 0:
+                at = b * tps if starts is None else starts[b]
+                pos = past[b] + torch.arange(new[b])
+                want[at:at + new[b]] = ((b * width + pos // 64) * 64 + pos % 64).to(I32)
+        assert torch.equal(slots, want)
+    good, n = [10, 64, 0, 7, 200], [top, 3, 0, 17, top]
+    starts = [2, 2 + top, 9 + top, 9 + top, 30 + top]
+    rows = 30 + 2 * top
+    check(good, n, starts, rows, 0, ())
+    check(good, n, None, 5 * top, top, ())
+    for past in (-1, -(2 ** 31), end - top + 1, 2 ** 31 - 1):
+        bad = [past] + good[1:]
+        check(bad, n, starts, rows, 0, (0,))
+        check(bad, n, None, 5 * top, top, (0,))
+    check(good, [top + 1, 3, 0, 17, top], None, 5 * top, top, (0,))          # more tokens than a padded row has
+    check(good, [top, 3, -4, 17, top], starts, rows, 0, (2,))
+    check(good, [top, 3, -4, 17, top], None, 5 * top, top, (2,))
+    check(good, n, starts, rows - 1, 0, (4,))                                # rows behind the last one
+    check(good, n, [-2] + starts[1:], rows, 0, (0,))                         # before the first one
