@@ -19,8 +19,8 @@
  * larger one, and the codes in front of them are rounded again at the new
  * scale; the first row of a block sets the scale afresh.  Rows behind the
  * last appended token are left as they were, and no result depends on them.
- * An infinite value counts as the largest finite bf16; NaN is stored as NaN
- * and counts for no scale.
+ * An infinite value counts as the largest finite bf16; NaN is stored as NaN,
+ * counts for no scale and reaches the tokens that see it, no others.
  *
  * One block may receive tokens of one sequence only in a call (blocks are not
  * shared between sequences that append).  2 KiB of cache hold one token of

@@ -951,6 +951,30 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         bp[i][e] = transpose8x8(pack_f16x2(p[0][i][e], kSets > 1 ? p[kSets - 1][i][e] : 0.f));
+    if (tail && ntok > 1) {
+      // a new token's NaN (no other code is not finite) must not meet p = 0 of the tokens in front of it: it goes
+      // to the outputs of those that see it, and the product takes a 0
+      bool moved = false;
+      for (int at = max(past + 1 - key0, 0); at < min(past + ntok - key0, kBlock); ++at) {
+        uint8_t *c0 = vc + lane * kBlock + at, *c1 = c0 + 32 * kBlock;  // dims lane, 32 + lane
+        const uint32_t n0 = __ballot_sync(0xffffffffu, (*c0 & 0x7f) == 0x7f);
+        const uint32_t n1 = __ballot_sync(0xffffffffu, (*c1 & 0x7f) == 0x7f);
+        if ((n0 | n1) == 0) continue;
+        moved = true;
+        if (n0 >> lane & 1) *c0 = 0;
+        if (n1 >> lane & 1) *c1 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // dim 16 i + 8 (e / 2) + g, vector 4 (e % 2) + t
+            const uint32_t bits = i < 2 ? n0 : n1;
+            if ((bits >> (16 * (i & 1) + 8 * (e >> 1) + g) & 1) && (4 * (e & 1) + t) >> 1 >= key0 + at - past)
+              o[i][e] = __int_as_float(0x7fffffff);
+          }
+      }
+      if (moved) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
+      __syncwarp();
+    }
     // O^T += V^T . P^T: rows g and g + 8 of m-tile i are dims 16 i + g and 16 i + 8 + g
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1262,6 +1286,7 @@ struct __align__(16) PrefillTail {
   uint64_t obar;                 // every product done (one commit)
   uint32_t tmem;
   int abort;
+  int nan_any, nan_key[kDim];    // first key with a NaN of V that not all rows of the tile see, per dim
 };
 constexpr int kPfSmem = 1024 + 2 * kPfOperand + 2 * kPfStages * kPfOperand + 2 * kPfRaw * kTile + (int)sizeof(PrefillTail);
 
@@ -1401,6 +1426,38 @@ __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
   }
 }
 
+// V's NaN at a key that only later rows of the query tile see (keys [first, end), counted from the V tile's first)
+// must not meet p = 0 of the others: the product takes a 0, and the rows that see the key get the NaN at the end.
+// One warp, on the codes in shared memory; two of 65 blocks for 64 x 128 tokens, 279 us with it and 273 without.
+// (Within the conversion 281, with a conversion loop of its own for such blocks 282.)
+__device__ __forceinline__ void hide_late_nans(uint8_t *tile, PrefillTail *tail, int key0, int first, int end) {
+  const int lane = threadIdx.x & 31;
+  const int at = 16 * (lane & 3);  // the lane's first key of the tile
+  auto from = [](int k, int i) { return k >= 4 * i + 4 ? 0u : (k <= 4 * i ? 0x80808080u : 0x80808080u << (8 * (k - 4 * i))); };
+  auto late = [&](int i) { return from(first - at, i) & ~from(end - at, i); };
+  auto nans = [](uint32_t x) { return (x & 0x7f7f7f7fu) + 0x01010101u; };  // top bit of each NaN's byte
+  const uint4 *piece = reinterpret_cast<const uint4 *>(tile) + lane;       // 32 i + lane: 16 tokens of dim 8 i + lane / 4
+  const uint32_t late0 = late(0), late1 = late(1), late2 = late(2), late3 = late(3);
+  uint32_t any = 0;
+#pragma unroll 4
+  for (int i = 0; i < 8; ++i) {
+    const uint4 x = piece[32 * i];
+    any |= (nans(x.x) & late0) | (nans(x.y) & late1) | (nans(x.z) & late2) | (nans(x.w) & late3);
+  }
+  if (!__any_sync(0xffffffffu, any != 0)) return;
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i) {  // word i % 4 of piece i / 4
+    uint32_t *word = reinterpret_cast<uint32_t *>(tile) + (32 * (i >> 2) + lane) * 4 + (i & 3);
+    const uint32_t z = nans(*word) & late(i & 3);
+    if (z == 0) continue;
+    atomicMin(&tail->nan_key[8 * (i >> 2) + (lane >> 2)], key0 + at + 4 * (i & 3) + ((__ffs(z) - 1) >> 3));
+    tail->nan_any = 1;
+    *word &= ~((z >> 7) * 0xffu);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
+  __syncwarp();
+}
+
 __device__ __forceinline__ float fmax3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
@@ -1504,9 +1561,18 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       ++issued;
     };
     for (int s = 0; s < kPfRaw; ++s) issue();
+    if (which) {
+      tail->nan_key[lane] = tail->nan_key[32 + lane] = 0x7fffffff;
+      if (lane == 0) tail->nan_any = 0;
+      __syncwarp();
+    }
+    const int whole = which ? (past + t0 + 1) / kBlock - j0 : nblk;  // V's blocks from here on hold keys that not all rows see
     for (int j = 0; j < nblk; ++j) {
       const int s = j % kPfStages, rs = j % kPfRaw;
       bool got = mbar_wait(smem_u32(&tail->raw[which][rs]), (j / kPfRaw) & 1, a.wait_ns);
+      if (j >= whole)
+        hide_late_nans(codes + rs * kTile, tail, (j0 + j) * kBlock, past + t0 + 1 - (j0 + j) * kBlock,
+                       last_key + 1 - (j0 + j) * kBlock);
       uint4 w[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint4 *>(codes + rs * kTile + (32 * i + lane) * 16);
@@ -1518,7 +1584,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
         tail->abort = 1;
         break;
       }
-      if (which && (j0 + j) * kBlock + kBlock - 1 > last_key) {
+      if (j >= whole && (j0 + j) * kBlock + kBlock - 1 > last_key) {
         // tokens past the tile's last key may hold anything (even NaN): p = 0 must not meet them
         const int n = last_key + 1 - (j0 + j) * kBlock - 16 * (lane & 3);
         auto mask = [&](int i) { return n >= 4 * i + 4 ? ~0u : (n <= 4 * i ? 0u : (1u << (8 * (n - 4 * i))) - 1u); };
@@ -1552,6 +1618,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       const int k = s + kPfRaw * ((issued - 1 - s) / kPfRaw);
       if (!mbar_wait(smem_u32(&tail->raw[which][s]), (k / kPfRaw) & 1, kDrainNs) && lane == 0) atomicOr(a.err, B2_DEV_TIMEOUT);
     }
+    if (which) asm volatile("bar.sync 2, 160;" ::: "memory");  // nan_key is complete
   } else if (warp == 4) {
     // ---------------- products: S_0, S_1, then per block P_j . V_j and S_{j+2}
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail->tmem)),
@@ -1747,6 +1814,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       tmem_fence_before();
       mbar_arrive(smem_u32(&tail->pready[j & 1]));
     }
+    asm volatile("bar.sync 2, 160;" ::: "memory");  // the V warp's nan_key
     if (!ok) {
       if (!tail->abort) atomicOr(a.err, B2_DEV_TIMEOUT);
       tail->abort = 1;
@@ -1755,6 +1823,10 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       const bool stop = __any_sync(0xffffffffu, tail->abort);
       float o[64];
       tmem_ld64(trow + 128, o);
+      if (tail->nan_any) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) o[c] = tail->nan_key[c] <= qpos ? __int_as_float(0x7fffffff) : o[c];
+      }
       const float unit = ex2(mo - m);  // the output in units of 2^m, as the sum
       if (stop) {
       } else if (pt.parts > 1) {

@@ -97,3 +97,86 @@ def test_slot_map_refuses_a_request_whole(cuda, many):
     check(good, [top, 3, -4, 17, top], None, 5 * top, top, (2,))
     check(good, n, starts, rows - 1, 0, (4,))                                # rows behind the last one
     check(good, n, [-2] + starts[1:], rows, 0, (0,))                         # before the first one
+
+
+# ------------------------------------------------------------------ NaN that a token does not see
+
+def _spoil(rows, at):
+    """NaN in the V of (sequence, token, KV head, dim) and, where dim is None, in one K value of the token's head."""
+    rows = rows.clone()
+    for b, t, h, d in at:
+        rows[b, t, (16 + h) * 64 + 5 if d is None else (24 + h) * 64 + d] = float("nan")
+    return rows
+
+
+def _check_nan(ref, table, past, rows, out, what):
+    """NaN where a visible token's V (or a visible K) is NaN; elsewhere the context, as if every NaN were a 0."""
+    q = ora.split(rows)[0]
+    n = rows.shape[0]
+    clean = ora.Cache(ref.k, ref.v, ref.ks, ref.vs)
+    bad_k, bad_v = clean.k.float().isnan(), clean.v.float().isnan()
+    clean.k.view(torch.uint8)[bad_k] = 0
+    clean.v.view(torch.uint8)[bad_v] = 0
+    marks = ora.Cache(ref.k, ref.v, ref.ks, ref.vs)
+    marks.k, marks.v = bad_k.float(), bad_v.float()
+    marks.ks, marks.vs = torch.ones_like(ref.ks), torch.ones_like(ref.vs)
+    k, v = ora.values(marks, table, past + n)                                   # [8, tokens, 64], 1 where NaN
+    sees = (torch.arange(past + n)[None] <= past + torch.arange(n)[:, None]).double()
+    nan = torch.einsum("tl,hld->thd", sees, v) + torch.einsum("tl,hl->th", sees, k.amax(-1))[..., None] > 0
+    nan = nan.repeat_interleave(2, 1)                                           # [n, 16, 64]
+    got = out.cpu()
+    assert torch.equal(got.isnan(), nan), what
+    want, mean, low = ora.attend(clean, table, past, q)
+    zero = torch.zeros((), dtype=torch.float64)
+    ora.check_context(torch.where(nan, zero.to(BF16), got), *(torch.where(nan, zero, x) for x in (want, mean, low)), what)
+
+
+@pytest.mark.parametrize("tokens", [2, 3, 4])
+@pytest.mark.parametrize("store", [True, False])
+def test_step_nan_of_a_later_token(cuda, tokens, store):
+    """A drafted token's NaN stays out of the tokens in front of it, across the edge of a block, too."""
+    a8, _, lib = _mods()
+    lens = [0, 61, 62, 63, 64, 200, 2000]
+    cache, ref = _build([n + (0 if store else tokens) for n in lens], cuda, seed=211, room=8)
+    tables = cache.block_tables()
+    rows = _rows(len(lens) * tokens, 212, cuda).view(len(lens), tokens, 2048)
+    last = tokens - 1
+    at = [(b, t, (b + t) % 8, (7 * b + 11 * t) % 64) for b in range(len(lens)) for t in range(1, tokens)]
+    at += [(1, last, 2, d) for d in range(64)] + [(3, last, 4, None), (5, last, 0, None), (5, 0, 6, 13), (6, last, 7, 63)]
+    rows = _spoil(rows, at)
+    if not store:       # the tokens are in the cache already
+        a8.append_kv8(rows.to(cuda), past_lens=_ints(lens, cuda), block_tables=tables, dev_err=_err(cuda),
+                      mode=lib.B2_STORE_KV, **cache.kv8())
+    out = torch.zeros(len(lens), tokens, 16, 64, dtype=BF16, device=cuda)
+    err = _err(cuda)
+    a8.decode_step_kv8(rows.to(cuda), _ints(lens, cuda), block_tables=tables, out=out, workspace=a8.workspace_kv8(cuda),
+                       dev_err=err, mode=lib.B2_STORE_KV if store else 0, **cache.kv8())
+    assert err.item() == 0
+    for b, p in enumerate(lens):
+        _, k, v = ora.split(rows[b])
+        ora.append(ref, tables[b].cpu(), p, k, v)
+    for b, p in enumerate(lens):
+        _check_nan(ref, tables[b].cpu(), p, rows[b], out[b], f"sequence {b}")
+
+
+@pytest.mark.parametrize("lens,tokens", [([0], 64), ([0, 37, 64], 130), ([5000], 70), ([1, 300] * 20, 65)])
+def test_prefill_nan_of_a_later_token(cuda, lens, tokens):
+    """The same for a chunk: one tile, several, keys split over CTAs, tiles sorted."""
+    a8, _, lib = _mods()
+    cache, ref = _build(lens, cuda, seed=213, room=tokens + 3)
+    tables = cache.block_tables()
+    rows = _rows(len(lens) * tokens, 214, cuda).view(len(lens), tokens, 2048)
+    at = []
+    for b in range(min(len(lens), 4)):
+        at += [(b, t, (b + t) % 8, (5 * t) % 64) for t in (0, 1, 17, 40, 62, 63)]
+        at += [(b, tokens - 1, 3, d) for d in range(64)] + [(b, tokens - 2, 5, None)]
+    rows = _spoil(rows, at)
+    out = torch.zeros(len(lens), tokens, 16, 64, dtype=BF16, device=cuda)
+    err = _err(cuda)
+    a8.prefill_kv8(rows.to(cuda), _ints(lens, cuda), block_tables=tables, out=out, workspace=a8.workspace_kv8(cuda),
+                   dev_err=err, mode=lib.B2_STORE_KV, **cache.kv8())
+    assert err.item() == 0
+    for b in range(min(len(lens), 6)):
+        _, k, v = ora.split(rows[b])
+        ora.append(ref, tables[b].cpu(), lens[b], k, v)
+        _check_nan(ref, tables[b].cpu(), lens[b], rows[b], out[b], f"sequence {b}")
