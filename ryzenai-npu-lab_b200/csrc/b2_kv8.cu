@@ -370,10 +370,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
 // The sum of p runs against the reference m (log2 units), moved only when a
 // score exceeds m + kSlack (a vote, no shuffles, in all other tiles).  The
 // products p * v scale are rounded to f16 against a reference of their own, mo:
-// g = v scale * 2^(m - mo) is 1 where the largest product so far is 1, and up to
-// kMaxGain needs no look at the tile (p * g <= 2^15); above, the tile's true
-// maximum decides whether mo moves.  f16 gives p 11 bits (bf16 would give 8)
-// down to 2^-14 of the largest product; what is below 2^-25 of it is lost.
+// g = v scale * 2^(m - mo) is 2^kTopLog2 where the largest product so far is, and
+// up to kMaxGain needs no look at the tile (p * g <= 2^15); above, the tile's
+// true maximum decides whether mo moves.  f16 gives p 11 bits (bf16 would give 8)
+// down to 2^-22 of the largest product; what is below 2^-33 of it is lost, so a
+// tail of 2^17 tokens loses at most 2^-16 of the largest product.  The room above
+// (2^7 of it) is shared by scores that rise and v scales that grow: less of it
+// means more looks, and in a prompt more passes over the output.
 //
 // Ends: a segment (sequence, head) inside one warp's range is written by that
 // warp.  Others leave partial states in shared memory, merged by the CTA after
@@ -389,9 +392,11 @@ constexpr int kMaxSeqs = 1024;   // sequences per launch (lengths and sums in sh
 constexpr int kSegmentCost = 2;  // tiles that the start and end of a segment weigh as
 constexpr int kMaxCtas = 256;
 constexpr uint64_t kDrainNs = 2000000000ull;
-constexpr float kSlack = 8.0f;          // log2 units that a score may exceed m by
-constexpr float kMaxGain = 128.0f;      // g without a look at the tile's maximum
-constexpr float kMaxGainLog2 = 7.0f;
+constexpr float kSlack = 5.0f;          // log2 units that a score may exceed m by
+constexpr float kTopLog2 = 8.0f;        // the largest product when mo moves
+constexpr float kMaxGainLog2 = 10.0f;   // g without a look at the tile's maximum
+constexpr float kMaxGain = 1024.0f;
+static_assert(kSlack + kMaxGainLog2 <= 15.0f && kTopLog2 <= kMaxGainLog2, "products of a weight stay in f16's range");
 constexpr float kMinGainLog2 = 60.0f;   // below 2^-60 the products' sum may underflow
 constexpr float kUnset = -1.0e30f;
 
@@ -928,8 +933,8 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
         float big = fmaxf(fmaxf(fmaxf(x[0], y[0]), fmaxf(x[1], y[1])), fmaxf(fmaxf(x[2], y[2]), fmaxf(x[3], y[3])));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        // the largest product so far at 1
-        const float n = big > 0.f ? fmaxf(mo[u], m[u] + vexp + __log2f(big * vmant)) : mo[u];
+        // the largest product so far at 2^kTopLog2
+        const float n = big > 0.f ? fmaxf(mo[u], m[u] + vexp + __log2f(big * vmant) - kTopLog2) : mo[u];
         const float again = ex2(mo[u] - n);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1755,8 +1760,8 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       const float lv = log2_scale(vs);
       float again = 1.f;
       if (m - mo + lv > kMaxGainLog2) {
-        // the largest product so far at 1
-        const float n = fmaxf(mo, top + lv);
+        // the largest product so far at 2^kTopLog2
+        const float n = fmaxf(mo, top + lv - kTopLog2);
         again = ex2(mo - n);
         mo = n;
       }

@@ -180,3 +180,56 @@ def test_prefill_nan_of_a_later_token(cuda, lens, tokens):
         _, k, v = ora.split(rows[b])
         ora.append(ref, tables[b].cpu(), lens[b], k, v)
         _check_nan(ref, tables[b].cpu(), lens[b], rows[b], out[b], f"sequence {b}")
+
+
+# ------------------------------------------------------------------ the ends of the ranges
+
+def _line(cuda, k0, v, room=8):
+    """One sequence whose keys are k0[j] in dim 0 and 0 elsewhere, with values v [8, n, 64]."""
+    _, pc, _ = _mods()
+    n = k0.numel()
+    cache = pc.PagedKVCache8(pc.blocks_for(n + room) + 1, n + room, device=cuda, fill=float("nan"))
+    cache.add_sequence(n)
+    k = torch.zeros(8, n, 64)
+    k[:, :, 0] = k0
+    cache.write_dense(0, 0, k.to(BF16), v.to(BF16))
+    return cache, ora.Cache.of(cache.kv8())
+
+
+def _contexts(cuda, cache, rows, past, prefill):
+    a8, _, lib = _mods()
+    t = rows.shape[0]
+    out = torch.zeros(1, t, 16, 64, dtype=BF16, device=cuda)
+    err = _err(cuda)
+    (a8.prefill_kv8 if prefill else a8.decode_step_kv8)(
+        rows[None].to(cuda), _ints([past], cuda), block_tables=cache.block_tables(), out=out,
+        workspace=a8.workspace_kv8(cuda), dev_err=err, mode=lib.B2_STORE_KV, **cache.kv8())
+    assert err.item() == 0
+    return out[0].cpu()
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("n", [500, 5000, 30000])
+def test_many_small_weights_beside_a_large_one(cuda, prefill, n):
+    """A token that takes the weight and has no value, and a flat tail at 2^-26 of it: the tail is the context.
+
+    A weight's f16 form is at least 2^-33 of the largest product, so rounding it costs at most 2^-33 of that per
+    unit of the code it multiplies: 2^-8 of check_context's `low`, which allows 2^-25."""
+    k0 = torch.full((n,), -2.0)
+    k0[0] = 16.0                                        # 18 nats above the others
+    g = torch.Generator().manual_seed(n)
+    v = 1.0 + 0.25 * torch.randn(8, n, 64, generator=g)
+    v[:, 0] = 0
+    cache, ref = _line(cuda, k0, v, room=40)
+    t = 33 if prefill else 3
+    rows = _rows(t, 221, cuda)
+    rows[:, :1024] = 0
+    rows[:, :1024:64] = 8.0                             # a query's score is its key's dim 0
+    rows[:, 1024:1536] = 0
+    rows[:, 1024:1536:64] = -2.0
+    out = _contexts(cuda, cache, rows, n, prefill)
+    table = cache.block_tables()[0].cpu()
+    q, k, val = ora.split(rows)
+    ora.append(ref, table, n, k, val)
+    want, mean, low = ora.attend(ref, table, n, q)
+    ora.check_context(out, want, mean, low * 2.0 ** -8)
