@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
 // lane, free of bank conflicts without a swizzle.
 //
 // Scales: a vector's scores are c * (q factor * k scale), the query scaled to
-// 2^8 so that f16 keeps all bf16 bits of values down to 2^-22 of its largest.
+// 2^14 so that f16 keeps all bf16 bits of values down to 2^-28 of its largest.
 // The sum of p runs against the reference m (log2 units), moved only when a
 // score exceeds m + kSlack (a vote, no shuffles, in all other tiles).  The
 // products p * v scale are rounded to f16 against a reference of their own, mo:
@@ -758,15 +758,15 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
         if (grp < 2) {
-          // the query with its largest value in [2^8, 2^9)
+          // the query with its largest value in [2^14, 2^15)
           int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
           e = e < -100 ? -100 : e;
-          const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
+          const float up = __uint_as_float(static_cast<uint32_t>(141 - e) << 23);
           const int v = 2 * i + grp;
           *reinterpret_cast<uint4 *>(&sh.row[warp].q[v][8 * j]) =
               make_uint4(pack_f16x2(y[0] * up, y[1] * up), pack_f16x2(y[2] * up, y[3] * up),
                          pack_f16x2(y[4] * up, y[5] * up), pack_f16x2(y[6] * up, y[7] * up));
-          if (j == 0) sh.factor[warp][v] = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
+          if (j == 0) sh.factor[warp][v] = __uint_as_float(static_cast<uint32_t>(113 + e) << 23) * a.scale_log2;
         }
       }
       __syncwarp();
@@ -1691,7 +1691,7 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     };
     int64_t id = pool_tile(lane);
     float2 scale = make_float2(__ldcg(a.k_scale + id), __ldcg(a.v_scale + id)), scale_next = scale;
-    // query rows: row r = (head of the pair) * 64 + token, its largest value at 2^8 in f16
+    // query rows: row r = (head of the pair) * 64 + token, its largest value at 2^14 in f16
     float factor = 0.f;
     {
       const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (row0 + t) * a.q_stride + (2 * h + hl) * kDim);
@@ -1707,8 +1707,8 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       }
       int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
       e = e < -100 ? -100 : e;
-      const float up = __uint_as_float(static_cast<uint32_t>(135 - e) << 23);
-      factor = __uint_as_float(static_cast<uint32_t>(119 + e) << 23) * a.scale_log2;
+      const float up = __uint_as_float(static_cast<uint32_t>(141 - e) << 23);
+      factor = __uint_as_float(static_cast<uint32_t>(113 + e) << 23) * a.scale_log2;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         float y[8];

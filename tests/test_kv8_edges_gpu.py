@@ -233,3 +233,26 @@ def test_many_small_weights_beside_a_large_one(cuda, prefill, n):
     ora.append(ref, table, n, k, val)
     want, mean, low = ora.attend(ref, table, n, q)
     ora.check_context(out, want, mean, low * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_query_values_far_apart(cuda, prefill):
+    """A query with one value 2^27 times the others, where every key is 0: the others decide."""
+    _, pc, _ = _mods()
+    lens = [3, 6, 9, 17]
+    for n in lens:
+        g = torch.Generator().manual_seed(n)
+        cache = pc.PagedKVCache8(3, 128, device=cuda, fill=float("nan"))
+        cache.add_sequence(n)
+        k = 2.0 * torch.randn(8, n, 64, generator=g)
+        k[:, :, 3] = 0
+        cache.write_dense(0, 0, k.to(BF16), torch.randn(8, n, 64, generator=g).to(BF16))
+        ref = ora.Cache.of(cache.kv8())
+        rows = _rows(6 if prefill else 4, 231 + n, cuda)
+        rows[:, 3:1024:64] = 2.0 ** 27
+        rows[:, 1024 + 3:1536:64] = 0
+        out = _contexts(cuda, cache, rows, n, prefill)
+        table = cache.block_tables()[0].cpu()
+        q, k, v = ora.split(rows)
+        ora.append(ref, table, n, k, v)
+        ora.check_context(out, *ora.attend(ref, table, n, q), f"{n} tokens")
