@@ -933,8 +933,9 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
         float big = fmaxf(fmaxf(fmaxf(x[0], y[0]), fmaxf(x[1], y[1])), fmaxf(fmaxf(x[2], y[2]), fmaxf(x[3], y[3])));
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        // the largest product so far at 2^kTopLog2
-        const float n = big > 0.f ? fmaxf(mo[u], m[u] + vexp + __log2f(big * vmant) - kTopLog2) : mo[u];
+        // the largest product so far at 2^kTopLog2 (p as small as 2^-126 may have one: g stays in fp32 all the same);
+        // where every p is 0, g may have left it
+        const float n = big > 0.f ? fmaxf(mo[u], m[u] + vexp + fmaxf(__log2f(big * vmant) - kTopLog2, -120.f)) : mo[u];
         const float again = ex2(mo[u] - n);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -942,7 +943,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
           o[i][2 + u] *= again;
         }
         mo[u] = n;
-        gain = vmant * ex2(m[u] - n + vexp);
+        gain = big > 0.f ? vmant * ex2(m[u] - n + vexp) : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

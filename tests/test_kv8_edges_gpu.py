@@ -256,3 +256,20 @@ def test_query_values_far_apart(cuda, prefill):
         q, k, v = ora.split(rows)
         ora.append(ref, table, n, k, v)
         ora.check_context(out, *ora.attend(ref, table, n, q), f"{n} tokens")
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+def test_huge_values_of_no_weight_behind_zeros(cuda, prefill):
+    """Values of 1e30 whose weight is 2^-230, in turn with blocks of zeros that have all the weight: no weight of 0
+    may meet a factor that left fp32."""
+    n = 64 * 600
+    even = torch.arange(n) // BLOCK % 2 == 0
+    k0 = torch.where(even, 10.0, -10.0)
+    v = 1e30 * torch.randn(8, n, 64, generator=torch.Generator().manual_seed(1))
+    v[:, even] = 0
+    cache, _ = _line(cuda, k0, v)
+    rows = torch.zeros(4, 2048, dtype=BF16)
+    rows[:, :1024:64] = 64.0
+    rows[:, 1024:1536:64] = -10.0
+    out = _contexts(cuda, cache, rows, n, prefill).float()
+    assert bool(torch.isfinite(out).all()) and float(out.abs().max()) <= 1e-30       # 1e30 x 2^-230 is 6e-40
