@@ -412,9 +412,9 @@ struct __align__(128) StepShared {
   static constexpr int kWarps = step_warps<kT>(), kStages = step_stages<kT>();
   static constexpr int kSets = (kT + 1) / 2;  // vectors of a lane
   static constexpr int kVecs = 4 * kSets;     // vectors: 2 * new token + head of the pair
-  struct State {  // unnormalised output, then (m, l), of every vector
+  struct State {  // output in units of 2^mo, and (m, l, mo, -), of every vector
     float o[kVecs][kDim];
-    float ml[kVecs][2];
+    float4 ref[kVecs];
   };
   uint8_t codes[kWarps][kStages][2 * kTile];
   union {
@@ -514,23 +514,37 @@ __device__ __forceinline__ void mma_codes(float c[4][4], const uint4 r[4][2], co
   }
 }
 
+// The (m, l, mo) of a partial state, written one by one: as one store it took four registers in a row for the whole
+// loop (prompt: 28 bytes of spills more, 289 us against 281 for 64 x 128 tokens).
+__device__ __forceinline__ void write_ref(float4 *ref, float m, float l, float mo) {
+  ref->x = m;
+  ref->y = l;
+  ref->z = mo;
+}
+
 // Sum of partial states of one new token: 16 lanes per head of the pair, 4 dims
-// each.  States come in groups of 16, lane i of the 16 holding state i's (m, l).
+// each.  States come in groups of 16, lane i of the 16 holding state i's (m, l,
+// mo).  Outputs keep the reference of their products, which the last division
+// takes with it: in units of 2^m a sum of values near fp32's largest leaves it.
 struct StateSum {
-  float m = kUnset, l = 0.f;
+  float m = kUnset, l = 0.f, mo = kUnset;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float c = 0.f;  // factor of this lane's state of the group
-  __device__ __forceinline__ void group(float2 ml) {
-    float top = ml.x;
+  __device__ __forceinline__ void group(float4 ref) {
+    float top = ref.x, top_o = ref.z;
 #pragma unroll
-    for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-    const float n = fmaxf(m, top), again = ex2(m - n);
-    m = n;
-    c = ex2(ml.x - n);
-    float s = ml.y * c;
+    for (int off = 1; off < 16; off <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      top_o = fmaxf(top_o, __shfl_xor_sync(0xffffffffu, top_o, off));
+    }
+    const float n = fmaxf(m, top), no = fmaxf(mo, top_o), again = ex2(mo - no);
+    float s = ref.y * ex2(ref.x - n);
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    l = fmaf(l, again, s);
+    l = fmaf(l, ex2(m - n), s);
+    m = n;
+    mo = no;
+    c = ex2(ref.z - no);
     o.x *= again;
     o.y *= again;
     o.z *= again;
@@ -545,7 +559,7 @@ struct StateSum {
   }
   // the two context rows
   __device__ __forceinline__ void write(uint16_t *out, int lane) const {
-    const float inv = 1.0f / l;
+    const float inv = ex2(mo - m) / l;
     *reinterpret_cast<uint2 *>(out + (lane >> 4) * kDim + 4 * (lane & 15)) =
         make_uint2(pack_bf16x2_rn(o.x * inv, o.y * inv), pack_bf16x2_rn(o.z * inv, o.w * inv));
   }
@@ -1015,20 +1029,16 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
 
     const bool last = blk + 1 == nblk;  // of the segment
     if (last || k + 1 == issued) {
-      // the output in units of 2^m, as the sum; dims 16 i + g, 16 i + 8 + g
-      float s[kSets];
 #pragma unroll
-      for (int u = 0; u < kSets; ++u) {
+      for (int u = 0; u < kSets; ++u)
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], off);
-        s[u] = ex2(mo[u] - m[u]);
-      }
       if (last && from_start) {
 #pragma unroll
         for (int u = 0; u < kSets; ++u) {
           const int v = 4 * u + t;
           if (v >= 2 * ntok) continue;
-          const float f = s[u] / l[u];
+          const float f = ex2(mo[u] - m[u]) / l[u];  // dims 16 i + g, 16 i + 8 + g
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             sh.row[warp].out[v][16 * i + g] = static_cast<uint16_t>(bf16_bits(o[i][u] * f));
@@ -1051,13 +1061,10 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
           const int v = 4 * u + t;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            st->o[v][16 * i + g] = o[i][u] * s[u];
-            st->o[v][16 * i + 8 + g] = o[i][2 + u] * s[u];
+            st->o[v][16 * i + g] = o[i][u];
+            st->o[v][16 * i + 8 + g] = o[i][2 + u];
           }
-          if (g == 0) {
-            st->ml[v][0] = m[u];
-            st->ml[v][1] = l[u];
-          }
+          if (g == 0) write_ref(&st->ref[v], m[u], l[u], mo[u]);
         }
         if (lane == 0) sh.open[warp][which] = b * kHkv + h;
       }
@@ -1109,9 +1116,9 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
           return (e & 1) ? reinterpret_cast<const State *>(sh.codes[e >> 1][0]) : &sh.head[e >> 1];
         };
         const int e = e0 + (lane & 15);
-        float2 ml = make_float2(kUnset, 0.f);
-        if (e < 2 * kWarps && (members >> e & 1)) ml = *reinterpret_cast<const float2 *>(state(e)->ml[vec]);
-        sum.group(ml);
+        float4 ref = make_float4(kUnset, 0.f, kUnset, 0.f);
+        if (e < 2 * kWarps && (members >> e & 1)) ref = state(e)->ref[vec];
+        sum.group(ref);
         for (uint32_t rest = members >> e0 & 0xffffu; rest; rest &= rest - 1) {
           const int i = __ffs(rest) - 1;
           sum.add(i, *reinterpret_cast<const float4 *>(&state(e0 + i)->o[vec][d]), lane);
@@ -1127,7 +1134,7 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
       const int cta = static_cast<int>(blockIdx.x);
       State *slot = slots + 2 * cta + (cta == cf ? 1 : 0);
       *reinterpret_cast<float4 *>(&slot->o[vec][d]) = sum.o;
-      if (d == 0) *reinterpret_cast<float2 *>(slot->ml[vec]) = make_float2(sum.m, sum.l);
+      if (d == 0) write_ref(&slot->ref[vec], sum.m, sum.l, sum.mo);
       __syncwarp();
       int32_t *counter = a.counters + cf * kMaxStepTokens + v;
       int arrived = 0;
@@ -1142,15 +1149,15 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
       for (int c0 = cf; c0 <= cl; c0 += 16) {
         // sixteen states' loads in flight together
         const int c = c0 + (lane & 15);
-        float2 ml = make_float2(kUnset, 0.f);
-        if (c <= cl) ml = __ldcg(reinterpret_cast<const float2 *>((slots + 2 * c + (c == cf ? 1 : 0))->ml[vec]));
+        float4 ref = make_float4(kUnset, 0.f, kUnset, 0.f);
+        if (c <= cl) ref = __ldcg(&(slots + 2 * c + (c == cf ? 1 : 0))->ref[vec]);
         float4 x[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int q = min(c0 + e, cl);
           x[e] = __ldcg(reinterpret_cast<const float4 *>(&(slots + 2 * q + (q == cf ? 1 : 0))->o[vec][d]));
         }
-        whole.group(ml);
+        whole.group(ref);
 #pragma unroll
         for (int e = 0; e < 16; ++e) whole.add(e, x[e], lane);  // factor 0 past the last state
       }
@@ -1296,9 +1303,9 @@ struct __align__(16) PrefillTail {
 };
 constexpr int kPfSmem = 1024 + 2 * kPfOperand + 2 * kPfStages * kPfOperand + 2 * kPfRaw * kTile + (int)sizeof(PrefillTail);
 
-struct PrefillState {  // unnormalised output and (m, l) of a query tile's rows over one CTA's blocks
+struct PrefillState {  // a query tile's rows over one CTA's blocks: output in units of 2^mo, and (m, l, mo, -)
   float o[2 * kBlock][kDim];
-  float ml[2 * kBlock][2];
+  float4 ref[2 * kBlock];
 };
 
 struct PrefillArgs {
@@ -1827,23 +1834,22 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
     } else if (warp_wait(smem_u32(&tail->obar), 0)) {
       tmem_fence_after();
       const bool stop = __any_sync(0xffffffffu, tail->abort);
+      PrefillState *st = pt.parts > 1 ? a.parts + ((static_cast<int64_t>(b) * a.tiles + tile) * kHkv + h) * a.nsplit + split
+                                      : nullptr;
+      if (st && !stop) write_ref(&st->ref[tid], m, l, mo);
+      const float inv = ex2(mo - m) / l;
       float o[64];
       tmem_ld64(trow + 128, o);
       if (tail->nan_any) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) o[c] = tail->nan_key[c] <= qpos ? __int_as_float(0x7fffffff) : o[c];
       }
-      const float unit = ex2(mo - m);  // the output in units of 2^m, as the sum
       if (stop) {
-      } else if (pt.parts > 1) {
-        PrefillState *st = a.parts + ((static_cast<int64_t>(b) * a.tiles + tile) * kHkv + h) * a.nsplit + split;
+      } else if (st) {
         float4 *dst = reinterpret_cast<float4 *>(st->o[tid]);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4)
-          dst[c >> 2] = make_float4(o[c] * unit, o[c + 1] * unit, o[c + 2] * unit, o[c + 3] * unit);
-        *reinterpret_cast<float2 *>(st->ml[tid]) = make_float2(m, l);
+        for (int c = 0; c < 64; c += 4) dst[c >> 2] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
       } else if (row_ok) {
-        const float inv = unit / l;
         uint4 *dst = reinterpret_cast<uint4 *>(a.out + ((row0 + t) * kHq + 2 * h + hl) * kDim);
 #pragma unroll
         for (int c = 0; c < 64; c += 8) {
@@ -1877,41 +1883,42 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const PrefillArgs a) {
   const int hl = r >> 6, t = r & 63;
   if (t >= pt.rows) return;
   const PrefillState *st = a.parts + (static_cast<int64_t>(b) * gridDim.x + blockIdx.x) * a.nsplit;
-  float m = kUnset, l = 0.f;
+  float m = kUnset, l = 0.f, mo = kUnset;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p0 = 0; p0 < pt.parts; p0 += 8) {
-    float2 ml[8];
-    float4 x[8];
-    float n = m;
+    float4 ref[8], x[8];
+    float n = m, no = mo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const PrefillState *q = st + min(p0 + e, pt.parts - 1);
-      ml[e] = __ldcg(reinterpret_cast<const float2 *>(q->ml[r]));
+      ref[e] = __ldcg(&q->ref[r]);
       x[e] = __ldcg(reinterpret_cast<const float4 *>(&q->o[r][d]));
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (p0 + e >= pt.parts) ml[e] = make_float2(kUnset, 0.f);
-      n = fmaxf(n, ml[e].x);
+      if (p0 + e >= pt.parts) ref[e] = make_float4(kUnset, 0.f, kUnset, 0.f);
+      n = fmaxf(n, ref[e].x);
+      no = fmaxf(no, ref[e].z);
     }
-    const float again = ex2(m - n);
+    l *= ex2(m - n);
+    const float again = ex2(mo - no);
     m = n;
-    l *= again;
+    mo = no;
     o.x *= again;
     o.y *= again;
     o.z *= again;
     o.w *= again;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = p0 + e < pt.parts ? ex2(ml[e].x - n) : 0.f;
-      l = fmaf(ml[e].y, f, l);
+      const float f = p0 + e < pt.parts ? ex2(ref[e].z - no) : 0.f;
+      l = fmaf(ref[e].y, ex2(ref[e].x - n), l);
       o.x = fmaf(x[e].x, f, o.x);
       o.y = fmaf(x[e].y, f, o.y);
       o.z = fmaf(x[e].z, f, o.z);
       o.w = fmaf(x[e].w, f, o.w);
     }
   }
-  const float inv = 1.0f / l;
+  const float inv = ex2(mo - m) / l;
   *reinterpret_cast<uint2 *>(a.out + ((pt.row + t) * kHq + 2 * h + hl) * kDim + d) =
       make_uint2(pack_bf16x2_rn(o.x * inv, o.y * inv), pack_bf16x2_rn(o.z * inv, o.w * inv));
 }

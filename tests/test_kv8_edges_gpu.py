@@ -273,3 +273,18 @@ def test_huge_values_of_no_weight_behind_zeros(cuda, prefill):
     rows[:, 1024:1536:64] = -10.0
     out = _contexts(cuda, cache, rows, n, prefill).float()
     assert bool(torch.isfinite(out).all()) and float(out.abs().max()) <= 1e-30       # 1e30 x 2^-230 is 6e-40
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("n", [500, 30000])
+def test_huge_values_of_even_weight(cuda, prefill, n):
+    """The mean of values of 1e36: their sum, which the states of a split sequence stand for, is over fp32's largest."""
+    v = 1e36 * (1.0 + 0.25 * torch.randn(8, n, 64, generator=torch.Generator().manual_seed(2)))
+    cache, ref = _line(cuda, torch.zeros(n), v, room=80)
+    rows = _rows(70 if prefill else 4, 241, cuda)
+    rows[:, 1536:2048] = (rows[:, 1536:2048].float() * 1e36).to(BF16)
+    out = _contexts(cuda, cache, rows, n, prefill)
+    table = cache.block_tables()[0].cpu()
+    q, k, val = ora.split(rows)
+    ora.append(ref, table, n, k, val)
+    ora.check_context(out, *ora.attend(ref, table, n, q))
