@@ -28,7 +28,13 @@ kv8=True keeps K and V in 8 bits (paged_cache.PagedKVCache8, half the cache
 bytes) with b2_kv8_decode_step in place of the bf16 step.  With pool_blocks as
 well, blocks are not reserved up front: device block tables (block_tables.py)
 take them from a pool of that many inside the captured token, so a pool smaller
-than max_batch full contexts serves sequences as they grow.
+than max_batch full contexts serves sequences as they grow.  A sequence that the
+pool cannot serve stays as it was: its token is not cached, its convolution
+states do not move and the next id returned for it is the token it was given,
+so feeding the returned ids back tries that token again.  `granted` says which
+sequences took the last token (int32 [max_batch] on the device; the logits of
+the others mean nothing), check() and generate() raise when any did not, and
+block_tables.release() returns the blocks of finished sequences.
 
 Weights come from a state dict with the Hugging Face parameter names
 (model.layers.{i}.self_attn.q_proj.weight, ...), e.g. a random-init model.
@@ -132,6 +138,7 @@ class LFM2DecodeRunner:
             self._new = torch.ones(max_batch, dtype=torch.int32, device=dev)
             self._plan = self.block_tables.plan(torch.zeros_like(self._new), tokens_per_seq=1)
             self._refused = torch.zeros(1, dtype=torch.int64, device=dev)
+            self.granted = self._plan.granted
         else:
             self.cache = (PagedKVCache8 if kv8 else PagedKVCache)(max_batch * per_seq, max_context, num_layers=n_att,
                                                                  device=dev)
@@ -149,6 +156,7 @@ class LFM2DecodeRunner:
                          for gq, gk in gammas]
         self.conv_state = torch.zeros(len(config.conv_layers), max_batch, config.hidden, config.conv_l,
                                       dtype=bf, device=dev)
+        self._conv_kept = None if self.block_tables is None else torch.empty_like(self.conv_state)
         self.past = torch.zeros(max_batch, dtype=torch.int32, device=dev) if self.block_tables is None \
             else self.block_tables.lens
         self.seq = torch.ones(max_batch, dtype=torch.int32, device=dev)
@@ -179,10 +187,15 @@ class LFM2DecodeRunner:
         if self.block_tables is not None:
             self.block_tables.plan(self._new, tokens_per_seq=1, out=self._plan)
             self._refused += (self._plan.granted == 0).sum()
+            self._conv_kept.copy_(self.conv_state)
         if self.fused_glue:
             self._token_fused()
         else:
             self._token_torch()
+        if self.block_tables is not None:       # what got no block stays as it was
+            got = self.granted > 0
+            torch.where(got[:, None, None], self.conv_state, self._conv_kept, out=self.conv_state)
+            torch.where(got, self.next_ids, self.ids, out=self.next_ids)
 
     def _attend(self, att: int, qkv: torch.Tensor) -> torch.Tensor:
         """Context [B, 16, 64] of attention layer `att` for the new tokens' projections."""
@@ -292,6 +305,7 @@ class LFM2DecodeRunner:
             # warm up on a side stream, then capture one token (state is
             # restored afterwards so the capture run does not count)
             saved = (self.past.clone(), self.conv_state.clone())  # restored after the capture run
+            refused = None if self.block_tables is None else self._refused.clone()
             s = torch.cuda.Stream(self.device)
             s.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(s):
@@ -304,6 +318,8 @@ class LFM2DecodeRunner:
                 self._token()
             self.past.copy_(saved[0])
             self.conv_state.copy_(saved[1])
+            if refused is not None:
+                self._refused.copy_(refused)
             self._graph = g
         self._graph.replay()
 
@@ -313,6 +329,7 @@ class LFM2DecodeRunner:
         """Forget every sequence (KV lengths and conv states back to zero)."""
         if self.block_tables is not None:
             self.block_tables.release(torch.ones(self.max_batch, dtype=torch.bool, device=self.device))
+            self._refused.zero_()
         self.past.zero_()
         self.conv_state.zero_()
         self.position = 0
@@ -339,12 +356,15 @@ class LFM2DecodeRunner:
         return out
 
     def generate(self, prompt_ids, new_tokens: int) -> torch.Tensor:
-        """Greedy decode: prefill the prompts, then feed back the argmax."""
+        """Greedy decode: prefill the prompts, then feed back the argmax.  With
+        pool_blocks, RuntimeError when the pool could not serve every token."""
         nxt = self.prefill(prompt_ids)
         out = [nxt.clone()]
         for _ in range(new_tokens - 1):
             nxt = self.step(nxt)
             out.append(nxt.clone())
+        if self.block_tables is not None:
+            self.check()
         return torch.stack(out, dim=1)
 
     def kv(self, att_index: int, seq: int, position: int):
