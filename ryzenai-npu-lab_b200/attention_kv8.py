@@ -20,6 +20,7 @@ import torch
 
 from . import _lib
 from .attention import D, EPS, HKV, HQ, MAX_STEP_TOKENS, QKV_WIDTH, SCALE, _need, _need_rope
+from .build import binding_matches
 from .paged_cache import BLOCK, PagedKVCache8
 from .rope import rope_table
 
@@ -28,14 +29,16 @@ NORM_ROPE_STORE = _lib.B2_NORM_QK | _lib.B2_ROPE_QK | _lib.B2_STORE_KV
 
 # The smallest calls are bound by the host.  The native binding (_b2torch, built
 # against the installed torch) checks a call's tensors and makes the library call
-# in one go, in half the time; where it is not built, or says None to an argument, the checks
-# below do the same: each is one comparison of what the tensor says about itself
+# in one go, in half the time; where it is not built (or for another torch), or says None to
+# an argument, the checks below do the same: each is one comparison of what the tensor says about itself
 # (its device by index), and the slow path that words the refusal is taken only
 # when one fails.
-try:
-    from . import _b2torch
-except ImportError:
-    _b2torch = None
+_b2torch = None
+if binding_matches():
+    try:
+        from . import _b2torch
+    except ImportError:
+        pass
 _bound = None       # the library whose functions the binding holds
 
 

@@ -10,6 +10,7 @@ import os
 import pathlib
 import shutil
 import subprocess
+import warnings
 
 PKG = pathlib.Path(__file__).resolve().parent
 ROOT = PKG.parent
@@ -17,6 +18,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libb2attn.so"
 BINDING = PKG / "_b2torch.so"
 BINDING_SOURCE = CSRC / "b2_torch.cpp"
+BINDING_HEADERS = [ROOT / "include" / "b2_kv8.h", ROOT / "include" / "b2_tables.h"]
 SOURCES = [CSRC / "b2_attn.cu", CSRC / "b2_block.cu", CSRC / "b2_gemm.cu",
            CSRC / "b2_kv8.cu", CSRC / "b2_tables.cu"]
 HEADERS = [ROOT / "include" / "b2_decode_attn.h", ROOT / "include" / "b2_block.h",
@@ -45,9 +47,30 @@ def needs_build(lib: pathlib.Path = LIB) -> bool:
     return any(p.stat().st_mtime > mtime for p in SOURCES + HEADERS)
 
 
+def binding_stamp() -> str:
+    """What the binding is compiled against and of no use without: this torch, this Python."""
+    import sysconfig
+
+    import torch
+    return f"b2torch for torch {torch.__version__} and {sysconfig.get_config_var('SOABI')}"
+
+
+def binding_matches(path: pathlib.Path = BINDING) -> bool:
+    """Whether the binding at `path` was compiled against the installed torch and this Python (it carries their
+    names, which are looked for before it is loaded)."""
+    return path.exists() and binding_stamp().encode() in path.read_bytes()
+
+
+def binding_needs_build() -> bool:
+    if not binding_matches(BINDING):
+        return True
+    mtime = BINDING.stat().st_mtime
+    return any(p.stat().st_mtime > mtime for p in (BINDING_SOURCE, *BINDING_HEADERS))
+
+
 def _start_binding(force: bool):
     """The compilation of the binding against the installed torch, started; None when up to date."""
-    if not force and BINDING.exists() and BINDING.stat().st_mtime > BINDING_SOURCE.stat().st_mtime:
+    if not force and not binding_needs_build():
         return None
     import sysconfig
 
@@ -57,6 +80,7 @@ def _start_binding(force: bool):
     lib = pathlib.Path(torch.__file__).parent / "lib"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DNDEBUG",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DB2_TORCH_STAMP="{binding_stamp()}"', f"-I{ROOT / 'include'}",
            *(f"-I{d}" for d in include_paths()), f"-I{sysconfig.get_paths()['include']}", str(BINDING_SOURCE),
            f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
     return tmp, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -72,13 +96,32 @@ def _finish_binding(started) -> None:
     os.replace(tmp, BINDING)
 
 
+def _without_binding(error: Exception) -> None:
+    """The package works without the binding, which halves the host's time of its smallest calls: its failure is a
+    warning, and a binding of other sources or another torch does not stay."""
+    try:
+        stale = binding_needs_build()
+    except ImportError:
+        stale = True
+    if stale:
+        BINDING.unlink(missing_ok=True)
+    warnings.warn(f"{BINDING.name} was not built, its calls go through Python: {error}", stacklevel=3)
+
+
 def build(force: bool = False, verbose: bool = False) -> pathlib.Path:
     """Compile the CUDA sources into libb2attn.so and the binding (each skipped when up to date)."""
-    binding = _start_binding(force)
+    binding = None
+    try:
+        binding = _start_binding(force)
+    except Exception as e:      # no torch, no compiler
+        _without_binding(e)
     try:
         return _build_library(force, verbose)
     finally:
-        _finish_binding(binding)
+        try:
+            _finish_binding(binding)
+        except Exception as e:
+            _without_binding(e)
 
 
 def _build_library(force: bool, verbose: bool) -> pathlib.Path:

@@ -7,7 +7,10 @@
 // accept what this path does not know, a tensor subclass for instance).
 //
 // The library's functions come by address (bind), so this module links neither
-// against it nor against CUDA.
+// against it nor against CUDA; their types come from the headers.  The module is
+// of use to the torch and the Python it was compiled against alone, whose names
+// it carries (stamp): build.py and attention_kv8.py look for them before it is
+// loaded.
 
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -16,26 +19,33 @@
 
 #include <initializer_list>
 
+#include "b2_kv8.h"
+#include "b2_tables.h"
+
 namespace {
+
+constexpr char kStamp[] = B2_TORCH_STAMP;
 
 constexpr int64_t kHq = 16, kHkv = 8, kDim = 64, kBlock = 64, kWidth = 2048;
 constexpr int kNorm = 1, kRope = 2, kStore = 4;
 
-using StepFn = int (*)(const void *, int64_t, int32_t, const void *, int32_t, const void *, const void *, const void *,
-                       float, const void *, const void *, int32_t, const void *, const void *, int32_t, void *, void *,
-                       void *, void *, int32_t, int32_t, float, int32_t, void *, void *, int64_t, void *, void *);
-using AppendFn = int (*)(const void *, int64_t, int32_t, const void *, const void *, const void *, const void *, int32_t,
-                         const void *, int32_t, const void *, const void *, float, const void *, const void *, int32_t,
-                         void *, void *, void *, void *, int32_t, void *, int32_t, void *, void *);
-using PrefillFn = int (*)(const void *, int64_t, int32_t, const void *, const void *, const void *, int32_t, const void *,
-                          int32_t, const void *, const void *, const void *, const void *, int32_t, int32_t, float,
-                          void *, void *, int64_t, void *, void *);
-using ExtendFn = int (*)(void *, int32_t, const void *, const void *, int32_t, const void *, const void *, const void *,
-                         int32_t, void *, void *, void *, void *, void *, void *, int32_t, int32_t, void *, void *);
+using StepFn = decltype(&b2_kv8_decode_step);
+using AppendFn = decltype(&b2_kv8_append);
+using PrefillFn = decltype(&b2_kv8_prefill_attn);
+using ExtendFn = decltype(&b2_tables_extend);
 StepFn g_step = nullptr;
 AppendFn g_append = nullptr;
 PrefillFn g_prefill = nullptr;
 ExtendFn g_extend = nullptr;
+
+// A tensor's address, for a parameter of any pointer type.
+struct Address {
+  void *p = nullptr;
+  template <class T>
+  operator T *() const {
+    return static_cast<T *>(p);
+  }
+};
 
 // The checks of one call: `ok` stays true while every argument is as expected.
 struct Args {
@@ -58,16 +68,16 @@ struct Args {
     if (t && (t->scalar_type() != type || !t->is_cuda() || t->get_device() != index || !t->is_contiguous())) ok = false;
     return ok ? t : nullptr;
   }
-  void *ptr(int i, at::ScalarType type, std::initializer_list<int64_t> sizes) {
+  Address ptr(int i, at::ScalarType type, std::initializer_list<int64_t> sizes) {
     const at::Tensor *t = plain(i, type);
     if (!t || !t->sizes().equals(at::IntArrayRef(sizes.begin(), sizes.size()))) {
       ok = false;
-      return nullptr;
+      return {};
     }
-    return t->data_ptr();
+    return {t->data_ptr()};
   }
-  void *ptr_or_null(int i, at::ScalarType type, std::initializer_list<int64_t> sizes) {
-    return at[i] == Py_None ? nullptr : ptr(i, type, sizes);
+  Address ptr_or_null(int i, at::ScalarType type, std::initializer_list<int64_t> sizes) {
+    return at[i] == Py_None ? Address{} : ptr(i, type, sizes);
   }
   int64_t whole(int i) {
     const int64_t v = PyLong_Check(at[i]) ? PyLong_AsLongLong(at[i]) : -1;
@@ -89,7 +99,7 @@ constexpr auto kF32 = at::kFloat;
 constexpr auto kE4m3 = at::kFloat8_e4m3fn;
 
 struct Cache {
-  void *k, *v, *ks, *vs;
+  Address k, v, ks, vs;
   int64_t blocks;
 };
 
@@ -109,7 +119,7 @@ Cache cache_args(Args &a, int i) {
 }
 
 struct QkArgs {
-  void *gq = nullptr, *gk = nullptr, *cos = nullptr, *sin = nullptr;
+  Address gq, gk, cos, sin;
   int64_t rows = 0;
 };
 
@@ -157,12 +167,12 @@ PyObject *step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const int64_t t = padded ? qkv->size(1) : a.whole(20), width = qkv->size(-1);
   const int64_t rows = padded ? b * t : qkv->size(0);
   if (t < 1 || t > 4 || width < kWidth || (padded && qkv->size(0) != b)) return not_here();
-  void *q = qkv->data_ptr(), *past = a.ptr(1, kI32, {b}), *table = a.ptr(6, kI32, {b, cols});
-  void *start = a.ptr_or_null(19, kI32, {b});
+  const Address q{qkv->data_ptr()}, past = a.ptr(1, kI32, {b}), table = a.ptr(6, kI32, {b, cols});
+  const Address start = a.ptr_or_null(19, kI32, {b});
   const Cache c = cache_args(a, 2);
-  void *out = padded ? a.ptr(7, kBf16, {b, t, kHq, kDim}) : a.ptr(7, kBf16, {rows, kHq, kDim});
+  const Address out = padded ? a.ptr(7, kBf16, {b, t, kHq, kDim}) : a.ptr(7, kBf16, {rows, kHq, kDim});
   const at::Tensor *work = a.plain(8, at::kByte);
-  void *err = a.ptr(9, kI32, {1}), *chunk = a.ptr_or_null(10, kI32, {b});
+  const Address err = a.ptr(9, kI32, {1}), chunk = a.ptr_or_null(10, kI32, {b});
   const QkArgs qk = qk_args(a, 11, mode);
   const float eps = a.number(16), scale = a.number(17);
   const int64_t stream = PyLong_AsLongLong(args[18]);
@@ -187,10 +197,10 @@ PyObject *prefill(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const at::Tensor *tables = a.plain(6, kI32);
   if (width < kWidth || !tables || tables->dim() != 2 || !a.plain(0, kBf16)) return not_here();
   const int64_t rows = qkv->numel() / width, b = tables->size(0), cols = tables->size(1), mode = a.whole(15);
-  void *past = a.ptr(1, kI32, {b}), *table = a.ptr(6, kI32, {b, cols});
+  const Address past = a.ptr(1, kI32, {b}), table = a.ptr(6, kI32, {b, cols});
   const Cache c = cache_args(a, 2);
   int64_t tokens;
-  void *out, *start = nullptr;
+  Address out, start;
   if (padded) {
     tokens = qkv->size(1);
     if (qkv->size(0) != b || args[19] != Py_None) return not_here();
@@ -202,16 +212,17 @@ PyObject *prefill(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (args[21] == Py_None) return not_here();
   }
   const at::Tensor *work = a.plain(8, at::kByte);
-  void *err = a.ptr(9, kI32, {1}), *chunk = a.ptr_or_null(10, kI32, {b});
+  const Address err = a.ptr(9, kI32, {1}), chunk = a.ptr_or_null(10, kI32, {b});
   const QkArgs qk = qk_args(a, 11, mode);
   const float eps = a.number(16), scale = a.number(17);
   const int64_t stream = PyLong_AsLongLong(args[18]);
-  void *slots = a.ptr_or_null(21, kI32, {rows}), *positions = a.ptr_or_null(22, kI32, {rows});
-  void *q_buf = a.ptr_or_null(23, kBf16, {rows, kHq, kDim});
+  const Address slots = a.ptr_or_null(21, kI32, {rows}), positions = a.ptr_or_null(22, kI32, {rows});
+  const Address q_buf = a.ptr_or_null(23, kBf16, {rows, kHq, kDim});
   if (!a.ok || !small({b, width, cols, c.blocks, qk.rows, rows, tokens}) ||
-      ((mode & (kNorm | kRope)) != 0) != (q_buf != nullptr))
+      ((mode & (kNorm | kRope)) != 0) != (q_buf.p != nullptr))
     return not_here();
-  void *st = reinterpret_cast<void *>(stream), *x = qkv->data_ptr();
+  void *st = reinterpret_cast<void *>(stream);
+  const Address x{qkv->data_ptr()};
   if (mode) {
     const int rc = g_append(x, width, static_cast<int32_t>(rows), slots, positions, past, chunk,
                             static_cast<int32_t>(tokens), table, static_cast<int32_t>(cols), qk.gq, qk.gk, eps, qk.cos,
@@ -219,7 +230,7 @@ PyObject *prefill(PyObject *, PyObject *const *args, Py_ssize_t n) {
                             static_cast<int32_t>(c.blocks), q_buf, static_cast<int32_t>(mode), err, st);
     if (rc) return PyLong_FromLong(rc);
   }
-  return PyLong_FromLong(g_prefill(q_buf ? q_buf : x, q_buf ? kHq * kDim : width, static_cast<int32_t>(rows), start,
+  return PyLong_FromLong(g_prefill(q_buf.p ? q_buf : x, q_buf.p ? kHq * kDim : width, static_cast<int32_t>(rows), start,
                                    past, chunk, static_cast<int32_t>(tokens), table, static_cast<int32_t>(cols), c.k,
                                    c.v, c.ks, c.vs, static_cast<int32_t>(c.blocks), static_cast<int32_t>(b), scale, out,
                                    work->data_ptr(), work->numel(), err, st));
@@ -237,16 +248,16 @@ PyObject *extend(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const at::Tensor *list = a.plain(2, kI32), *slot_rows = a.plain(10, kI32);
   if (!list || !slot_rows) return not_here();
   const int64_t blocks = list->numel(), rows = slot_rows->numel(), tokens = a.whole(12);
-  void *table = a.ptr(0, kI32, {b, cols}), *held = a.ptr(1, kI32, {b}), *free_list = a.ptr(2, kI32, {blocks});
-  void *count = a.ptr(3, kI32, {1}), *past = a.ptr(4, kI32, {b}), *fresh = a.ptr(5, kI32, {b});
-  void *held_out = a.ptr_or_null(6, kI32, {b}), *count_out = a.ptr_or_null(7, kI32, {1});
-  void *granted = a.ptr(8, kI32, {b}), *start = a.ptr(9, kI32, {b}), *slots = a.ptr(10, kI32, {rows});
-  void *positions = a.ptr(11, kI32, {rows}), *err = a.ptr(13, kI32, {1});
+  const Address table = a.ptr(0, kI32, {b, cols}), held = a.ptr(1, kI32, {b}), free_list = a.ptr(2, kI32, {blocks});
+  const Address count = a.ptr(3, kI32, {1}), past = a.ptr(4, kI32, {b}), fresh = a.ptr(5, kI32, {b});
+  const Address held_out = a.ptr_or_null(6, kI32, {b}), count_out = a.ptr_or_null(7, kI32, {1});
+  const Address granted = a.ptr(8, kI32, {b}), start = a.ptr(9, kI32, {b}), slots = a.ptr(10, kI32, {rows});
+  const Address positions = a.ptr(11, kI32, {rows}), err = a.ptr(13, kI32, {1});
   const int64_t stream = PyLong_AsLongLong(args[14]);
   if (!a.ok || !small({b, cols, blocks, rows, tokens})) return not_here();
   return PyLong_FromLong(g_extend(table, static_cast<int32_t>(cols), held, free_list, static_cast<int32_t>(blocks), count,
-                                  past, fresh, static_cast<int32_t>(b), held_out ? held_out : held,
-                                  count_out ? count_out : count, granted, start, slots, positions,
+                                  past, fresh, static_cast<int32_t>(b), held_out.p ? held_out : held,
+                                  count_out.p ? count_out : count, granted, start, slots, positions,
                                   static_cast<int32_t>(rows), static_cast<int32_t>(tokens), err,
                                   reinterpret_cast<void *>(stream)));
 }
@@ -286,4 +297,11 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_b2torch", "native binding of li
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__b2torch(void) { return PyModule_Create(&g_module); }
+PyMODINIT_FUNC PyInit__b2torch(void) {
+  PyObject *m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "stamp", kStamp) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
