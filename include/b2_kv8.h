@@ -72,8 +72,8 @@ int b2_kv8_append(const uint16_t *qkv, int64_t row_stride, int32_t rows,
  * qkv        rows of row_stride, `rows` of them; token t of sequence b is row
  *            row_start[b] + t (NULL: b * tokens + t).  chunk_lens[b] (0 ..
  *            tokens; NULL: tokens) tokens are there; a sequence with none is
- *            skipped, one that would leave the rows is refused
- *            (B2_DEV_BAD_LENGTH).
+ *            skipped whatever its length and row, one that would leave the
+ *            rows is refused (B2_DEV_BAD_LENGTH).
  * out        bf16 [rows][16][64]; rows of no token are left as they were.
  * workspace  b2_kv8_workspace_bytes() bytes, 16-byte aligned, zeroed once; a
  *            call that completes leaves it ready for the next.  Calls that

@@ -600,9 +600,9 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     if (b < a.batch) {
       const int past = __ldcg(a.past_lens + b), ntok = a.chunk_lens ? __ldcg(a.chunk_lens + b) : a.tokens;
       const int64_t first = row_of(b);
-      const bool fits = past >= 0 && ntok >= 0 && ntok <= a.tokens &&
-                        static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock &&
-                        first >= 0 && first + ntok <= a.rows;
+      const bool fits = ntok == 0 || (past >= 0 && ntok > 0 && ntok <= a.tokens &&
+                                      static_cast<int64_t>(past) + ntok <= static_cast<int64_t>(a.max_blocks) * kBlock &&
+                                      first >= 0 && first + ntok <= a.rows);
       if (!fits && blockIdx.x == 0) atomicOr(a.err, B2_DEV_BAD_LENGTH);
       if (fits && ntok > 0) n = ((past + ntok + kBlock - 1) / kBlock + kSegmentCost) * kHkv;
       sh.past[b] = past;

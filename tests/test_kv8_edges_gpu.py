@@ -288,3 +288,48 @@ def test_huge_values_of_even_weight(cuda, prefill, n):
     q, k, val = ora.split(rows)
     ora.append(ref, table, n, k, val)
     ora.check_context(out, *ora.attend(ref, table, n, q))
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 70])
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_sequence_of_no_token_is_skipped_whatever_its_lengths(cuda, tokens, packed):
+    """Slots of a batch that nobody uses: their lengths, rows and tables may be left over."""
+    a8, _, lib = _mods()
+    lens, chunk = [70, -9, 10 ** 6, 5, 2 ** 31 - 1], [tokens, 0, 0, 1, 0]
+    live = (0, 3)
+    cache, ref = _build([max(0, min(n, 200)) for n in lens], cuda, seed=251, room=80)
+    tables = cache.block_tables()
+    tables[1] = -1
+    tables[2] = 1 << 30
+    b = len(lens)
+    rows = _rows(b * tokens, 252, cuda)
+    starts = [tokens * i for i in range(b)]
+    err, out = _err(cuda), torch.full((b * tokens, 16, 64), -7.0, dtype=BF16, device=cuda)
+    args = dict(block_tables=tables, workspace=a8.workspace_kv8(cuda), dev_err=err, mode=lib.B2_STORE_KV,
+                chunk_lens=_ints(chunk, cuda), **cache.kv8())
+    shape = (rows.to(cuda), out)
+    if packed:
+        args |= dict(row_start=_ints([0, -50, 10 ** 6, starts[3], 2 ** 31 - 1], cuda), max_tokens=tokens)
+    else:
+        shape = (rows.to(cuda).view(b, tokens, 2048), out.view(b, tokens, 16, 64))
+    if tokens > 4:
+        if packed:
+            slots = [-1] * (b * tokens)
+            for i in live:
+                for t in range(chunk[i]):
+                    p = lens[i] + t
+                    slots[starts[i] + t] = int(tables[i, p // BLOCK]) * BLOCK + p % BLOCK
+            args["slots"] = _ints(slots, cuda)
+        a8.prefill_kv8(shape[0], _ints(lens, cuda), out=shape[1], **args)
+    else:
+        a8.decode_step_kv8(shape[0], _ints(lens, cuda), out=shape[1], **args)
+    assert err.item() == 0
+    seen = torch.zeros(b * tokens, dtype=torch.bool)
+    for i in live:
+        n, r = chunk[i], starts[i]
+        q, k, v = ora.split(rows[r:r + n])
+        ora.append(ref, tables[i].cpu(), lens[i], k, v)
+        ora.check_context(out[r:r + n], *ora.attend(ref, tables[i].cpu(), lens[i], q), f"sequence {i}")
+        seen[r:r + n] = True
+    assert bool((out[~seen.to(cuda)] == -7.0).all())
+    assert ref.same_as(cache.kv8())
