@@ -57,7 +57,8 @@ enum {
   B2_DEV_BAD_BLOCK = 1,     /* block table entry outside [0, num_blocks) */
   B2_DEV_BAD_LENGTH = 2,    /* length/position outside the block table */
   B2_DEV_BAD_POSITION = 4,  /* RoPE position outside the cos/sin table */
-  B2_DEV_TIMEOUT = 8        /* an mbarrier wait gave up (no hang) */
+  B2_DEV_TIMEOUT = 8,       /* an mbarrier wait gave up (no hang) */
+  B2_DEV_BAD_SLOT = 16      /* rows of one block that do not follow one another */
 };
 
 /* b2_append_rope mode bits */

@@ -44,7 +44,12 @@ extern "C" {
  * The rows' places, one of
  *   slots      int32 [rows]: block * 64 + row of the block (what
  *              b2_tables_extend and b2_slot_map write); a negative slot is a
- *              row to skip.  Rows of one block are adjacent and ascending.
+ *              row to skip.  Rows of one block follow one another without
+ *              skipped rows between them, at consecutive slots: one warp
+ *              writes them.  Others of the block, as far as skipped rows or a
+ *              jump part them from its first ones, are not stored
+ *              (B2_DEV_BAD_SLOT); rows of a block that those of another block
+ *              part are a race that no check finds.
  *              positions int32 [rows] are the RoPE positions (B2_ROPE_QK).
  *   slots NULL rows = batch * tokens, row b * tokens + t at position
  *              past_lens[b] + t, for t < chunk_lens[b] (NULL: tokens), through

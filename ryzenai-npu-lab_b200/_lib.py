@@ -20,6 +20,7 @@ B2_DEV_BAD_BLOCK = 1
 B2_DEV_BAD_LENGTH = 2
 B2_DEV_BAD_POSITION = 4
 B2_DEV_TIMEOUT = 8
+B2_DEV_BAD_SLOT = 16
 
 B2_NORM_QK = 1
 B2_ROPE_QK = 2
@@ -37,6 +38,7 @@ DEV_ERR_NAMES = {
     B2_DEV_BAD_LENGTH: "length or position outside the block table",
     B2_DEV_BAD_POSITION: "RoPE position outside the cos/sin table",
     B2_DEV_TIMEOUT: "a bounded device wait ran out",
+    B2_DEV_BAD_SLOT: "rows of one block that do not follow one another",
 }
 
 _p = ctypes.c_void_p

@@ -146,7 +146,9 @@ def append_kv8(qkv: torch.Tensor, *, k_pool: torch.Tensor | None = None, v_pool:
                eps: float = EPS, stream: torch.cuda.Stream | None = None) -> None:
     """q/k RMSNorm + RoPE and the quantised append of k, v (b2_kv8_append).
     qkv: bf16 [rows, >= 2048] with `slots` int32 [rows] (and `positions` for
-    RoPE) as the table builder writes them, a negative slot skipping its row;
+    RoPE) as the table builder writes them, a negative slot skipping its row
+    (rows of one block follow one another, at consecutive slots and without
+    skipped rows between them; later ones are refused in dev_err);
     or [batch, tokens, >= 2048] with past_lens and block_tables.  q_out: bf16
     [rows, 16, 64] normalised and rotated query."""
     if not isinstance(qkv, torch.Tensor) or qkv.dim() not in (2, 3) or qkv.shape[-1] < QKV_WIDTH:

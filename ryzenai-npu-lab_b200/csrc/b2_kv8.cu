@@ -165,6 +165,17 @@ __device__ __forceinline__ int row_place(const AppendArgs &a, int row, int &posi
   return blk * kBlock + static_cast<int>(pos % kBlock);
 }
 
+// One warp: the nearest row up to r with a slot lies in block `blk`.
+__device__ __forceinline__ bool block_in_front(const AppendArgs &a, int r, int blk) {
+  const int lane = threadIdx.x & 31;
+  for (; r >= 0; r -= 32) {
+    const int s = r - lane >= 0 ? a.slots[r - lane] : kNoSlot;
+    const uint32_t there = __ballot_sync(0xffffffffu, s >= 0 && s < a.num_blocks * kBlock);
+    if (there) return __shfl_sync(0xffffffffu, s, __ffs(there) - 1) / kBlock == blk;
+  }
+  return false;
+}
+
 // One CTA per window of rows and pair of heads, warp = (KV head, K or V).  A run
 // is a sequence of adjacent rows that go to adjacent slots of one block; the
 // warps of the window that holds its first row quantise the whole run, each for
@@ -233,8 +244,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Append
   const int here = lane < kWindow ? sh.slot[1 + lane] : kNoSlot, before = lane < kWindow ? sh.slot[lane] : kNoSlot;
   uint32_t starts = __ballot_sync(0xffffffffu, here >= 0 && (before < 0 || before + 1 != here || here % kBlock == 0));
   for (; starts; starts &= starts - 1) {
-    const int i0 = __ffs(starts), s0 = sh.slot[i0];
+    const int i0 = __ffs(starts), s0 = sh.slot[i0], front = sh.slot[i0 - 1];
     const int blk = s0 / kBlock, r0 = s0 % kBlock;
+    // rows of this block in front of the run belong to another warp, which writes its scale: refused
+    if (front >= 0 ? front / kBlock == blk : a.slots && r0 > 0 && block_in_front(a, row0 + i0 - 3, blk)) {
+      if (threadIdx.x == 0 && blockIdx.y == 0) atomicOr(a.err, B2_DEV_BAD_SLOT);
+      continue;
+    }
     // rows that follow: 1 + lane, 33 + lane behind the first
     const uint32_t m0 = __ballot_sync(0xffffffffu, r0 + 1 + lane < kBlock && sh.slot[i0 + 1 + lane] == s0 + 1 + lane);
     const uint32_t m1 = __ballot_sync(0xffffffffu, r0 + 33 + lane < kBlock && sh.slot[i0 + 33 + lane] == s0 + 33 + lane);

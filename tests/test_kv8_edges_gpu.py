@@ -333,3 +333,44 @@ def test_a_sequence_of_no_token_is_skipped_whatever_its_lengths(cuda, tokens, pa
         seen[r:r + n] = True
     assert bool((out[~seen.to(cuda)] == -7.0).all())
     assert ref.same_as(cache.kv8())
+
+
+@pytest.mark.parametrize("gap", [1, 7, 31, 32, 33, 300])
+def test_rows_of_a_block_behind_skipped_rows_are_refused(cuda, gap):
+    """Skipped rows stand between runs of different blocks; a block whose rows they part is written by its first run
+    alone, whichever rows of the call share a CTA."""
+    a8, _, lib = _mods()
+    lens = [100, 30, 64, 7]
+    cache, ref = _build(lens, cuda, seed=261, room=100)
+    tables = cache.block_tables()
+
+    def slots_of(b, t0, n):
+        return [int(tables[b, p // BLOCK]) * BLOCK + p % BLOCK for p in range(lens[b] + t0, lens[b] + t0 + n)]
+    skip = [-1] * gap
+    parts = [(0, 0, 5), (0, 5, 3), (1, 0, 34), (1, 34, 20), (2, 0, 2), (3, 0, 1)]
+    #        100..104   105..107    30..63     64..: own    another sequence's blocks
+    slots, kept, row = [], [], 3
+    for b, t0, n in parts:
+        slots += skip + slots_of(b, t0, n)
+        row = len(slots) - n
+        if (b, t0) != (0, 5):                               # goes on in block 1 of sequence 0
+            kept.append((b, t0, n, row))
+    rows = _rows(len(slots), 262, cuda, sigma=20.0)
+    err = _err(cuda)
+    q_out = torch.full((len(slots), 16, 64), -7.0, dtype=BF16, device=cuda)
+    a8.append_kv8(rows.to(cuda), slots=_ints(slots, cuda), dev_err=err, q_out=q_out, mode=lib.B2_STORE_KV, **cache.kv8())
+    assert err.item() == lib.B2_DEV_BAD_SLOT
+    for b, t0, n, r in kept:
+        _, k, v = ora.split(rows[r:r + n])
+        ora.append(ref, tables[b].cpu(), lens[b] + t0, k, v)
+    assert ref.same_as(cache.kv8())
+    # in one piece nothing is refused
+    cache2, ref2 = _build(lens, cuda, seed=261, room=100)
+    slots = slots_of(0, 0, 8) + skip + slots_of(1, 0, 54) + slots_of(2, 0, 2) + skip
+    rows = _rows(len(slots), 263, cuda)
+    err.zero_()
+    a8.append_kv8(rows.to(cuda), slots=_ints(slots, cuda), dev_err=err, mode=lib.B2_STORE_KV, **cache2.kv8())
+    for b, n, r in ((0, 8, 0), (1, 54, 8 + gap), (2, 2, 62 + gap)):
+        _, k, v = ora.split(rows[r:r + n])
+        ora.append(ref2, tables[b].cpu(), lens[b], k, v)
+    assert err.item() == 0 and ref2.same_as(cache2.kv8())
