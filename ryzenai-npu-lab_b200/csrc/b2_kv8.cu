@@ -1457,8 +1457,9 @@ __device__ void prefill_job(const PrefillArgs &a, int job, PrefillJob &chosen) {
 
 // V's NaN at a key that only later rows of the query tile see (keys [first, end), counted from the V tile's first)
 // must not meet p = 0 of the others: the product takes a 0, and the rows that see the key get the NaN at the end.
-// One warp, on the codes in shared memory; two of 65 blocks for 64 x 128 tokens, 279 us with it and 273 without.
-// (Within the conversion 281, with a conversion loop of its own for such blocks 282.)
+// One warp, on the codes in shared memory; two of 65 blocks for 64 x 128 tokens, 283 us with it and 279 without.
+// (Within the conversion 3 us more, as were a conversion loop of its own for such blocks and a look between two runs of
+// the loop; unrolled, its cold instructions cost a call of one tile 0.15 us.)
 __device__ __forceinline__ void hide_late_nans(uint8_t *tile, PrefillTail *tail, int key0, int first, int end) {
   const int lane = threadIdx.x & 31;
   const int at = 16 * (lane & 3);  // the lane's first key of the tile
@@ -1468,7 +1469,7 @@ __device__ __forceinline__ void hide_late_nans(uint8_t *tile, PrefillTail *tail,
   const uint4 *piece = reinterpret_cast<const uint4 *>(tile) + lane;       // 32 i + lane: 16 tokens of dim 8 i + lane / 4
   const uint32_t late0 = late(0), late1 = late(1), late2 = late(2), late3 = late(3);
   uint32_t any = 0;
-#pragma unroll 4
+#pragma unroll 1
   for (int i = 0; i < 8; ++i) {
     const uint4 x = piece[32 * i];
     any |= (nans(x.x) & late0) | (nans(x.y) & late1) | (nans(x.z) & late2) | (nans(x.w) & late3);
@@ -1856,10 +1857,6 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
       const float inv = ex2(mo - m) / l;
       float o[64];
       tmem_ld64(trow + 128, o);
-      if (tail->nan_any) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c) o[c] = tail->nan_key[c] <= qpos ? __int_as_float(0x7fffffff) : o[c];
-      }
       if (stop) {
       } else if (st) {
         float4 *dst = reinterpret_cast<float4 *>(st->o[tid]);
@@ -1873,6 +1870,15 @@ __global__ void __launch_bounds__(kPfThreads, 2) kv8_prefill_kernel(const Prefil
 #pragma unroll
           for (int e = 0; e < 8; ++e) o8[e] = o[c + e] * inv;
           dst[c >> 3] = pack8(o8);
+        }
+      }
+      if (tail->nan_any && !stop) {
+        // over what was written: a loop of few instructions (as part of the output it cost every call 0.4 us)
+#pragma unroll 1
+        for (int c = 0; c < 64; ++c) {
+          if (tail->nan_key[c] > qpos) continue;
+          if (st) st->o[tid][c] = __int_as_float(0x7fffffff);
+          else if (row_ok) a.out[((row0 + t) * kHq + 2 * h + hl) * kDim + c] = 0x7fff;
         }
       }
     } else {
