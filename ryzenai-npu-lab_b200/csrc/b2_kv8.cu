@@ -990,8 +990,17 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
     if (tail && ntok > 1) {
       // a new token's NaN (no other code is not finite) must not meet p = 0 of the tokens in front of it: it goes
       // to the outputs of those that see it, and the product takes a 0
-      bool moved = false;
-      for (int at = max(past + 1 - key0, 0); at < min(past + ntok - key0, kBlock); ++at) {
+      bool moved = false, look = !(a.mode & B2_STORE_KV);  // (their v is in registers, or in the cache alone)
+      if (!look) {
+        uint32_t nans = 0;  // top bit of a bf16 that is a NaN
+#pragma unroll
+        for (int i = 1; i < kT; ++i) {
+          if (i >= ntok) break;
+          for (const uint32_t w : {fresh[i].x, fresh[i].y, fresh[i].z, fresh[i].w}) nans |= (w & 0x7fff7fffu) + 0x007f007fu;
+        }
+        look = __any_sync(0xffffffffu, grp == 3 && (nans & 0x80008000u));
+      }
+      for (int at = max(past + 1 - key0, 0); look && at < min(past + ntok - key0, kBlock); ++at) {
         uint8_t *c0 = vc + lane * kBlock + at, *c1 = c0 + 32 * kBlock;  // dims lane, 32 + lane
         const uint32_t n0 = __ballot_sync(0xffffffffu, (*c0 & 0x7f) == 0x7f);
         const uint32_t n1 = __ballot_sync(0xffffffffu, (*c1 & 0x7f) == 0x7f);
@@ -1008,8 +1017,10 @@ __global__ void __launch_bounds__(step_warps<kT>() * 32, 1) kv8_step_kernel(cons
               o[i][e] = __int_as_float(0x7fffffff);
           }
       }
-      if (moved) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
-      __syncwarp();
+      if (moved) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
+        __syncwarp();
+      }
     }
     // O^T += V^T . P^T: rows g and g + 8 of m-tile i are dims 16 i + g and 16 i + 8 + g
 #pragma unroll
