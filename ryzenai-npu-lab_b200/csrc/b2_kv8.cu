@@ -1280,9 +1280,9 @@ int launch_step(StepArgs a, cudaStream_t st) {
 // are K-major.  S and P are double-buffered, as the operands' rings are, so
 // conversion, products and softmax of different blocks overlap.
 //
-// 64 sequences, 128 new tokens over 128-8192 cached: 286 us with the append (14),
+// 64 sequences, 128 new tokens over 128-8064 cached: 286 us with the append (14),
 // against 84 us of products at the matrix rate and 50 us of bytes.  Profiled:
-// exponentials 52 % of their pipe, matrix pipe 25 %, DRAM 13 %, issue 50 %: what
+// exponentials 50 % of their pipe, matrix pipe 24 %, DRAM 13 %, issue 49 %: what
 // bounds it is the chain of a block (S, 64 scores to registers, maximum, 64
 // exponentials, P to tensor memory), about 1.1 us, of which two CTAs per SM run
 // side by side.  Three CTAs per SM with half the stages (344 us against 331 then),
